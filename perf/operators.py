@@ -353,7 +353,7 @@ def prepare(case, seed):
                 decode.kv4_append_gpu(k, v, seq.to(torch.int32), pos.to(torch.int32), cache, table)
             n = case["queries"]
             state["q_offsets"] = _int32([n * b for b in range(case["batch"] + 1)])
-            state["workspace"] = decode.AttentionWorkspace(q.shape[0], case["q_heads"], dim, "cuda")
+            state["workspace"] = decode.AttentionWorkspace(dim, "cuda")
             state["out"] = torch.empty_like(q)
         else:
             cache = _PlainCache(pages, page, kh, dim)
