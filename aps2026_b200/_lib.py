@@ -26,6 +26,10 @@ B2_CHECK_GATHER = 1
 B2_CHECK_ROPE = 2
 B2_CHECK_COMBINE = 4
 B2_CHECK_ATTENTION = 8
+B2_CHECK_KV4 = 64
+
+B2_DTYPE_F32, B2_DTYPE_BF16 = 0, 1
+B2_GATES_EQUAL, B2_GATES_SOFTMAX = 0, 1
 
 _vp, _sz, _f32, _u32 = C.c_void_p, C.c_size_t, C.c_float, C.c_uint32
 
@@ -60,6 +64,16 @@ SIGNATURES: dict[str, tuple] = {
     "b2_write_outputs": (C.c_int, [C.c_char_p, _vp, _sz, _sz, C.c_int, _vp]),
     "b2_selfcheck_exp": (C.c_int, [_u32, _u32, _vp, _vp, _vp]),
     "b2_selfcheck_wait": (C.c_int, [C.c_uint64]),
+    "b2_kv4_page_bytes": (C.c_int, [_sz, _sz, _sz, _vp]),
+    "b2_kv4_append": (C.c_int, [_vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _u32, _sz, _vp, _vp, _vp,
+                                _vp, _sz, _vp, _vp]),
+    "b2_kv4_read": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _u32, _vp]),
+    "b2_attention_kv4_workspace_size": (C.c_int, [_sz, _vp]),
+    "b2_attention_kv4": (C.c_int, [_vp, _sz, _sz, _vp, _u32, _sz, _sz, _vp, _vp, _sz, _sz, _f32, _sz, _sz, _vp,
+                                   _vp, _sz, _vp]),
+    "b2_moe_decode_workspace_size": (C.c_int, [_sz, _sz, _vp]),
+    "b2_moe_decode": (C.c_int, [_vp, _sz, _u32, _vp, _sz, _sz, _sz, _sz, _f32, _f32, _u32, _vp, _vp, _u32, _vp, _sz,
+                                _vp, _sz, _vp]),
     # struct arguments (b2_prefill_shape / _layer / _work) are passed by address
     "b2_prefill_layers": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp,
                                     _vp, _vp]),

@@ -92,6 +92,8 @@ int take_check_moe(cudaStream_t, unsigned int*);
 int take_check_attention(cudaStream_t, unsigned int*);
 int take_check_trie(cudaStream_t, unsigned int*);
 int take_check_selfcheck(cudaStream_t, unsigned int*);
+int take_check_kv4_cache(cudaStream_t, unsigned int*);
+int take_check_attention_kv4(cudaStream_t, unsigned int*);
 
 }  // namespace b2
 
@@ -113,6 +115,8 @@ int b2_device_status(uint32_t* status_out, b2_stream_t stream) {
     if ((rc = b2::take_check_attention(s, &acc)) != B2_OK) return rc;
     if ((rc = b2::take_check_trie(s, &acc)) != B2_OK) return rc;
     if ((rc = b2::take_check_selfcheck(s, &acc)) != B2_OK) return rc;
+    if ((rc = b2::take_check_kv4_cache(s, &acc)) != B2_OK) return rc;
+    if ((rc = b2::take_check_attention_kv4(s, &acc)) != B2_OK) return rc;
     *status_out = acc;
     return B2_OK;
 }

@@ -26,13 +26,13 @@
 #include <string>
 
 #include "fastexp.cuh"
+#include "route_pick.cuh"
 #include "rowload.cuh"
 
 namespace b2 {
 namespace {
 
 constexpr int kTile = 256;          // tokens per routing tile = threads per CTA
-constexpr int kMaxExperts = 32;
 
 // Histogram row stride: E rounded up to a power of two >= 4, so a tile's
 // counts are whole 16-byte vectors.
@@ -60,58 +60,13 @@ struct RouteArgs {
     std::size_t tiles;
 };
 
-// sign(s) * floorf(|s| / quantum + 0.5f) * quantum, the reference's
-// canonicalisation (src/tensor.cu:1301-1305), with every operation rounded
-// separately (no contraction is possible in the reference expression).
-__device__ __forceinline__ float quantize(float s, float quantum) {
-    const float r = __fmul_rn(floorf(__fadd_rn(__fdiv_rn(fabsf(s), quantum), 0.5f)), quantum);
-    return s < 0.0f ? -r : r;
-}
-
-// The two experts of token t, first | second << 8, as k_moe_top2 picks
-// them (src/tensor.cu:1299-1328): the first scan takes an expert when its
-// quantized score beats the best so far by more than tie_eps, the second
-// scan does the same skipping the first pick; also stored to routes[t].
+// The two experts of token t (route_pick.cuh), also stored to routes[t].
 __device__ __forceinline__ unsigned pick_top2(const RouteArgs& a, std::size_t t) {
     const unsigned E = static_cast<unsigned>(a.E);
     float sc[kMaxExperts];
-    const float* row = a.logits + t * a.E;
-    if ((E & 3u) == 0 && aligned16(row)) {
-#pragma unroll
-        for (unsigned e = 0; e < kMaxExperts; e += 4)
-            if (e < E) {
-                const float4 v = ld_stream(reinterpret_cast<const float4*>(row + e));
-                sc[e] = v.x; sc[e + 1] = v.y; sc[e + 2] = v.z; sc[e + 3] = v.w;
-            }
-    } else {
-#pragma unroll
-        for (unsigned e = 0; e < kMaxExperts; ++e)
-            if (e < E) sc[e] = __ldg(row + e);
-    }
-    int first = -1;
-    float first_value = -3.402823466e+38F;
-#pragma unroll
-    for (unsigned e = 0; e < kMaxExperts; ++e)
-        if (e < E) {
-            sc[e] = quantize(sc[e], a.quantum);
-            if (first < 0 || sc[e] > __fadd_rn(first_value, a.tie_eps)) {
-                first = static_cast<int>(e);
-                first_value = sc[e];
-            }
-        }
-    int second = -1;
-    float second_value = -3.402823466e+38F;
-#pragma unroll
-    for (unsigned e = 0; e < kMaxExperts; ++e)
-        if (e < E && static_cast<int>(e) != first) {
-            if (second < 0 || sc[e] > __fadd_rn(second_value, a.tie_eps)) {
-                second = static_cast<int>(e);
-                second_value = sc[e];
-            }
-        }
-    const unsigned short pair =
-        static_cast<unsigned short>(first) | (static_cast<unsigned short>(second) << 8);
-    reinterpret_cast<unsigned short*>(a.routes)[t] = pair;
+    load_scores(a.logits + t * a.E, E, sc);
+    const unsigned pair = top2_of_scores(sc, E, a.quantum, a.tie_eps);
+    reinterpret_cast<unsigned short*>(a.routes)[t] = static_cast<unsigned short>(pair);
     return pair;
 }
 

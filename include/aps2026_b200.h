@@ -86,6 +86,7 @@ const char* b2_last_error(void);
 #define B2_CHECK_ATTENTION 8u
 #define B2_CHECK_TRIE 16u
 #define B2_CHECK_WAIT 32u    /* a bounded wait for a bulk copy gave up; the CTA stopped */
+#define B2_CHECK_KV4 64u     /* a position, page, length or query offset of the 4-bit cache */
 int b2_device_status(uint32_t* status_out, b2_stream_t stream);
 
 /* ---- embedding / row gather ---------------------------------------------- */
@@ -353,6 +354,138 @@ int b2_moe_combine(const float* expert_out, size_t expert_rows,
  * src/tensor.cu:3236-3242; kernel k_add :1990-1993).
  */
 int b2_add(float* a, const float* b, size_t n, b2_stream_t stream);
+
+/* ---- decode: a 4-bit paged KV cache and the attention over it ------------------- */
+/*
+ * What carries a prefilled model on, token by token; no reference counterpart
+ * (the reference recomputes every prompt from its tokens). All three entry
+ * points describe the cache with b2_kv4_cache.
+ */
+
+/* Element type of an operator's activations or weights. */
+#define B2_DTYPE_F32 0u
+#define B2_DTYPE_BF16 1u
+
+/*
+ * Keys and values of `seqs` sequences in pages of page_size positions. Page
+ * page_table[s * max_pages + p / page_size] holds position p of sequence s;
+ * entries that no call reaches may hold anything. A page keeps, for each KV
+ * head, page_size rows of codes of K, of V, of parameters of K and of V;
+ * b2_kv4_page_bytes gives its size. A row of head_dim values has one 4-bit
+ * code c per value and, per 64 dimensions, a step s and a minimum m in bf16:
+ * the value held is s * c + m.
+ * page_size: a power of two, 8 at least; head_dim 64 or 128; data 16-byte
+ * aligned, pages * b2_kv4_page_bytes long; pages and page_table in device
+ * memory.
+ */
+typedef struct b2_kv4_cache {
+    void* data;
+    size_t pages, page_size, kv_heads, head_dim;
+    const uint32_t* page_table; /* [seqs, max_pages] */
+    size_t seqs, max_pages;
+} b2_kv4_cache;
+
+int b2_kv4_page_bytes(size_t page_size, size_t kv_heads, size_t head_dim, size_t* bytes);
+
+/*
+ * Appends rows to the cache, rotating keys (and queries) on the way. Row r is
+ * position row_pos[r] of sequence row_seq[r]; row_seq[r] = 0xFFFFFFFF marks a
+ * padding row. For each row:
+ *   q_out[r] = rotate(q[r], row_pos[r])          (q == NULL: no queries)
+ *   cache K at (row_seq[r], row_pos[r]) = round4(rotate(k[r], row_pos[r]))
+ *   cache V likewise = round4(v[r])
+ * rotate: the rotate-half pairs (j, j + head_dim/2) of b2_rope with the
+ * tables of b2_rope_table ([table_rows, head_dim/2]), each product and sum
+ * rounded to fp32 on its own; cos_table == NULL: no rotation.
+ * round4, per 64 dimensions: m = bf16(min), s = bf16(max(max - m, 0) *
+ * fp32(1/15)), c = clamp(rint((x - m) * (1/s)), 0, 15), 1/s taken as 0 for
+ * s < 2^-126. A NaN or infinity makes its 64 dimensions read back as NaN.
+ * q, k, v: `dtype`, [rows, heads, head_dim] with strides in elements between
+ * rows and between heads (the dimensions of a head adjacent), so slices of a
+ * fused projection need no copy; q_out: `dtype`, [rows, q_heads, head_dim]
+ * contiguous, may be q when q is contiguous. Rows must not share a position.
+ * Reported through b2_device_status and skipped (q_out zero where the
+ * rotation could not be had): a position past table_rows (B2_CHECK_ROPE); a
+ * sequence, position or page outside the cache (B2_CHECK_KV4). q_out of
+ * padding rows is zero.
+ */
+int b2_kv4_append(const void* q, size_t q_row_stride, size_t q_head_stride,
+                  size_t q_heads, void* q_out, const void* k,
+                  size_t k_row_stride, size_t k_head_stride, const void* v,
+                  size_t v_row_stride, size_t v_head_stride, uint32_t dtype,
+                  size_t rows, const uint32_t* row_seq,
+                  const uint32_t* row_pos, const float* cos_table,
+                  const float* sin_table, size_t table_rows,
+                  const b2_kv4_cache* cache, b2_stream_t stream);
+
+/*
+ * Reads rows back as the values the cache holds: k_out, v_out ([rows,
+ * kv_heads, head_dim] contiguous, `dtype`) = the keys and values at
+ * (row_seq[r], row_pos[r]); what the tree attention of a prompt that
+ * continues a cached prefix takes as K and V. Rows outside the cache are
+ * reported (B2_CHECK_KV4) and zero; padding rows (0xFFFFFFFF) are zero.
+ */
+int b2_kv4_read(const b2_kv4_cache* cache, const uint32_t* row_seq,
+                const uint32_t* row_pos, size_t rows, void* k_out,
+                void* v_out, uint32_t dtype, b2_stream_t stream);
+
+/*
+ * Attention of each sequence's newest rows over its cached keys and values:
+ *   out[r, h] = sum_j softmax_j(scale * q[r, h] . k[j, g]) v[j, g],
+ * g = h / (q_heads / kv_heads), over the visible keys j. lens[s] counts the
+ * cached positions of sequence s, those of its query rows included;
+ * q_offsets [seqs + 1] gives sequence s the query rows q_offsets[s] ..
+ * q_offsets[s + 1], the last of which is at position lens[s] - 1 and the
+ * others right before it (q_offsets == NULL: one row per sequence). Key j is
+ * visible at position p when j <= p and (p - j < window or j < sinks);
+ * window == 0: every j <= p. A row that sees no key is zero. Pages of keys
+ * that no row sees are not touched.
+ * q: `dtype` with strides as in b2_kv4_append; out: `dtype`, [rows, q_heads,
+ * head_dim] contiguous. max_queries and max_len bound the query rows and the
+ * length of a sequence (they size the launch).
+ * workspace: b2_attention_kv4_workspace_size bytes, 16-byte aligned, all zero
+ * before its first use; every call leaves it ready for the next. Calls that
+ * overlap on the GPU must not share it.
+ * Reported through b2_device_status (B2_CHECK_KV4): a sequence with more
+ * than max_queries query rows or offsets outside [0, rows] (its rows are not
+ * written); a length above max_len or the table's reach (its rows are zero);
+ * a page outside the cache (its keys are not seen).
+ */
+int b2_attention_kv4_workspace_size(size_t head_dim, size_t* bytes);
+int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride,
+                     void* out, uint32_t dtype, size_t rows, size_t q_heads,
+                     const uint32_t* q_offsets, const uint32_t* lens,
+                     size_t max_queries, size_t max_len, float scale,
+                     size_t window, size_t sinks, const b2_kv4_cache* cache,
+                     void* workspace, size_t workspace_bytes,
+                     b2_stream_t stream);
+
+/* ---- decode: the expert layer for a few tokens ----------------------------------- */
+
+#define B2_GATES_EQUAL 0u   /* 0.5 each, as b2_moe_combine weighs them */
+#define B2_GATES_SOFTMAX 1u /* softmax over the two picked router logits */
+
+/*
+ * A whole mixture-of-experts layer for T <= 128 tokens (one decode step), in
+ * two launches; no reference counterpart. Token t goes to the two experts
+ * that b2_moe_route picks from logits[t, :] (same quantum and tie_eps rule):
+ *   out[t] = sum over its experts e, ascending, of gate(t, e) *
+ *            w_down[e] (silu(w_gate_up[e][:I] x[t]) * (w_gate_up[e][I:] x[t]))
+ * x [T, ld_x >= H] and out [T, ld_out >= H]: x_dtype; logits [T, E] fp32,
+ * 2 <= E <= 32; w_gate_up [E, 2I, H] and w_down [E, H, I] contiguous:
+ * w_dtype. Sums in fp32; the products are those of the inputs as they are.
+ * out may not overlap x. T > 128: B2_ERR_UNSUPPORTED (route with
+ * b2_moe_route and run the experts as grouped products).
+ * workspace: b2_moe_decode_workspace_size bytes, 16-byte aligned; no
+ * initialisation. Calls that overlap on the GPU must not share it.
+ */
+int b2_moe_decode_workspace_size(size_t T, size_t I, size_t* bytes);
+int b2_moe_decode(const void* x, size_t ld_x, uint32_t x_dtype,
+                  const float* logits, size_t T, size_t H, size_t E, size_t I,
+                  float quantum, float tie_eps, uint32_t gates,
+                  const void* w_gate_up, const void* w_down, uint32_t w_dtype,
+                  void* out, size_t ld_out, void* workspace,
+                  size_t workspace_bytes, b2_stream_t stream);
 
 /* ---- prefix-trie dedup ------------------------------------------------------ */
 
