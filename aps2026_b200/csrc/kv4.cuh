@@ -133,7 +133,7 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
         for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(p[i]);
     }
 }
-// Rounded once to the element type, 16-byte aligned.
+// Rounded once to the element type, to 16-byte aligned global memory.
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
     st_plain(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
     st_plain(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
