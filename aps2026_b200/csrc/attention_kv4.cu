@@ -775,7 +775,11 @@ attention_kv4_shares(AttnKv4Args a) {
     // ---- this CTA's share of the list (pair-major, then head, then unit) ----
     const unsigned long long work = all_units * heads;
     unsigned long long share = (work + gridDim.x - 1) / gridDim.x;
-    if (share < kWarps) share = kWarps;
+    // short contexts: not less than a pair, up to a unit per warp, so that a
+    // pair is not cut for nothing
+    const unsigned long long per_pair = (work + static_cast<unsigned long long>(pairs) * heads - 1) /
+                                        (static_cast<unsigned long long>(pairs) * heads);
+    share = max(share, min(per_pair, static_cast<unsigned long long>(kWarps)));
     unsigned long long at = blockIdx.x * share;
     const unsigned long long stop = min(at + share, work);
     if (at >= stop) return;
@@ -856,12 +860,13 @@ cudaError_t launch_attention(const AttnKv4Args& a, cudaStream_t s) {
     const std::size_t smem = sizeof(Smem<D>);
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    // no more CTAs than there can be shares of kWarps units
+    // a CTA per pair at least, and no more than there can be shares of kWarps units
     const std::size_t keys = a.window ? std::min<std::size_t>(a.max_len, std::size_t(a.window) + a.sinks + a.max_queries)
                                       : a.max_len;
-    const std::size_t units = (keys + kStep - 1) / kStep * a.cache.seqs * a.tiles * a.cache.kv_heads;
-    std::size_t grid = std::min<std::size_t>(2 * sm_count(), kMaxGrid);
-    grid = std::max<std::size_t>(1, std::min(grid, (units + kWarps - 1) / kWarps));
+    const std::size_t pairs = static_cast<std::size_t>(a.cache.seqs) * a.tiles * a.cache.kv_heads;
+    const std::size_t units = (keys + kStep - 1) / kStep * pairs;
+    const std::size_t grid = std::min<std::size_t>(std::min<std::size_t>(2 * sm_count(), kMaxGrid),
+                                                   std::max(pairs, (units + kWarps - 1) / kWarps));
     return launch_pdl(kernel, static_cast<unsigned>(grid), kWarps * 32, smem, s, a);
 }
 

@@ -197,12 +197,19 @@ kv4_read_rows(Kv4View cache, const std::uint32_t* row_seq, const std::uint32_t* 
     }
 }
 
+// Grid of 256-thread CTAs for a grid-stride loop: at most 8 per SM, all that
+// an SM can hold (no occupancy query: it costs a decode step 1 us a call).
+inline unsigned full_grid(std::size_t ctas) {
+    const std::size_t most = static_cast<std::size_t>(sm_count()) * 8;
+    return static_cast<unsigned>(ctas < most ? ctas : most);
+}
+
 template <typename T, unsigned D>
 void launch_append(const AppendArgs& a, bool vec, cudaStream_t s) {
     const std::size_t units = static_cast<std::size_t>(a.rows) * (a.q_heads + 2 * a.cache.kv_heads);
     const std::size_t ctas = (units + 256 / (D / 16) - 1) / (256 / (D / 16));
     auto kernel = vec ? kv4_append_rows<T, D, true> : kv4_append_rows<T, D, false>;
-    launch_pdl(kernel, wave_grid(reinterpret_cast<const void*>(kernel), 256, 0, ctas), 256, 0, s, a);
+    launch_pdl(kernel, full_grid(ctas), 256, 0, s, a);
 }
 
 template <typename T, unsigned D>
@@ -211,8 +218,7 @@ void launch_read(const Kv4View& c, const std::uint32_t* seq, const std::uint32_t
     const std::size_t units = static_cast<std::size_t>(rows) * 2 * c.kv_heads;
     const std::size_t ctas = (units + 256 / (D / 8) - 1) / (256 / (D / 8));
     auto kernel = kv4_read_rows<T, D>;
-    launch_pdl(kernel, wave_grid(reinterpret_cast<const void*>(kernel), 256, 0, ctas), 256, 0, s, c, seq, pos, rows,
-               static_cast<T*>(k), static_cast<T*>(v));
+    launch_pdl(kernel, full_grid(ctas), 256, 0, s, c, seq, pos, rows, static_cast<T*>(k), static_cast<T*>(v));
 }
 
 }  // namespace

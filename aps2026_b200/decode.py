@@ -12,6 +12,7 @@ device: what is out of range there is skipped and reported by
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -32,6 +33,11 @@ class _CacheStruct(C.Structure):
                 ("max_pages", C.c_size_t)]
 
 
+# The same struct as bytes: a call's own immutable copy, cheaper to make.
+_pack_cache = struct.Struct("@PNNNNPNN").pack
+assert struct.calcsize("@PNNNNPNN") == C.sizeof(_CacheStruct)
+
+
 def _dtype(t: torch.Tensor, what: str) -> int:
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -49,9 +55,12 @@ def _index(t: torch.Tensor, n: int, device, what: str) -> int:
 def _heads(t: torch.Tensor, rows: int, heads: int, dim: int, device, what: str) -> tuple[int, int, int]:
     """Address and strides of [rows, heads, dim] activations whose last
     dimension is contiguous (slices of a fused projection are)."""
-    if t.shape != (rows, heads, dim) or t.device != device or (t.stride(2) != 1 and t.numel()):
-        raise InvalidArgument(f"{what}: expected [{rows}, {heads}, {dim}] on {device} with a contiguous last dimension")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    if t.shape != (rows, heads, dim) or t.device != device:
+        raise InvalidArgument(f"{what}: expected [{rows}, {heads}, {dim}] on {device}")
+    by_row, by_head, by_dim = t.stride()
+    if by_dim != 1 and rows:
+        raise InvalidArgument(f"{what}: the last dimension must be contiguous")
+    return t.data_ptr(), by_row, by_head
 
 
 def _whole(t: torch.Tensor, shape: tuple, like: torch.Tensor, what: str) -> int:
@@ -64,10 +73,10 @@ def _on_gpu(device: torch.device) -> int:
     """The current stream of `device`, which must be the current device."""
     if device.type != "cuda":
         raise InvalidArgument("tensor is not on a CUDA device")
-    stream = torch.cuda.current_stream()
-    if stream.device != device:
-        raise InvalidArgument(f"tensors are on {device}, the current device is {stream.device}")
-    return stream.cuda_stream
+    if device.index != torch.cuda.current_device():
+        raise InvalidArgument(f"tensors are on {device}, the current device is {torch.cuda.current_device()}")
+    # torch.cuda.current_stream().cuda_stream without the 3 us of building a Stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class KVCache4:
@@ -82,12 +91,13 @@ class KVCache4:
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.data = torch.zeros(pages, n.value, dtype=torch.uint8, device=device)
 
-    def _struct(self, page_table: torch.Tensor) -> _CacheStruct:
+    def _struct(self, page_table: torch.Tensor) -> bytes:
         if (page_table.dim() != 2 or page_table.dtype not in _INDEX or page_table.device != self.data.device
                 or not page_table.is_contiguous()):
             raise InvalidArgument("page_table: expected contiguous 32-bit indices [seqs, max_pages] on the cache's device")
-        return _CacheStruct(self.data.data_ptr(), self.pages, self.page_size, self.kv_heads, self.head_dim,
-                            page_table.data_ptr(), page_table.shape[0], page_table.shape[1])
+        seqs, max_pages = page_table.shape
+        return _pack_cache(self.data.data_ptr(), self.pages, self.page_size, self.kv_heads, self.head_dim,
+                           page_table.data_ptr(), seqs, max_pages)
 
 
 def kv4_append_gpu(k, v, row_seq, row_pos, cache: KVCache4, page_table, q=None, q_out=None, cos=None,
@@ -126,7 +136,7 @@ def kv4_append_gpu(k, v, row_seq, row_pos, cache: KVCache4, page_table, q=None, 
         cp, sp, positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
     _check(_lib.lib().b2_kv4_append(
         qp, qr, qh, q_heads, qo, kp, kr, kh, vp, vr, vh, dtype, rows, _index(row_seq, rows, device, "row_seq"),
-        _index(row_pos, rows, device, "row_pos"), cp, sp, positions, C.byref(cache._struct(page_table)), stream),
+        _index(row_pos, rows, device, "row_pos"), cp, sp, positions, cache._struct(page_table), stream),
         "kv4_append_gpu")
 
 
@@ -141,7 +151,7 @@ def kv4_read_gpu(cache: KVCache4, page_table, row_seq, row_pos, k_out, v_out) ->
     if k_out.device != device:
         raise InvalidArgument("kv4_read: outputs must be on the cache's device")
     _check(_lib.lib().b2_kv4_read(
-        C.byref(cache._struct(page_table)), _index(row_seq, rows, device, "row_seq"),
+        cache._struct(page_table), _index(row_seq, rows, device, "row_seq"),
         _index(row_pos, rows, device, "row_pos"), rows, _whole(k_out, shape, k_out, "kv4_read k_out"),
         _whole(v_out, shape, k_out, "kv4_read v_out"), _dtype(k_out, "kv4_read k_out"), stream), "kv4_read_gpu")
 
@@ -186,7 +196,7 @@ def attention_kv4_gpu(q, cache: KVCache4, page_table, lens, out, q_offsets=None,
         qp, qr, qh, _whole(out, q.shape, q, "attention_kv4 out"), _dtype(q, "attention_kv4 q"), rows, q_heads,
         None if q_offsets is None else _index(q_offsets, seqs + 1, device, "q_offsets"),
         _index(lens, seqs, device, "lens"), max_queries, max_len, dim ** -0.5 if scale is None else scale, window,
-        sinks, C.byref(cache._struct(page_table)), ws.buf.data_ptr(), ws.bytes, stream), "attention_kv4_gpu")
+        sinks, cache._struct(page_table), ws.buf.data_ptr(), ws.bytes, stream), "attention_kv4_gpu")
 
 
 class MoeWorkspace:
