@@ -29,6 +29,7 @@
 // the start of another; parts meet in the workspace, where the last CTA to
 // arrive adds them in the list's order, so results repeat bit for bit.
 #include <algorithm>
+#include <cmath>
 
 #include <cuda_fp16.h>
 
@@ -39,7 +40,7 @@ namespace {
 
 constexpr unsigned kWarps = 8;           // warps per CTA
 constexpr unsigned kStep = 32;           // positions per warp step
-constexpr unsigned kRows = 8;            // query rows per tile
+constexpr unsigned kRows = 8;            // query rows per tile, at most
 constexpr unsigned kPairCache = 256;     // pairs whose sizes a CTA keeps
 constexpr unsigned kMaxGrid = 2 * 160;   // CTAs the workspace is sized for
 constexpr float kNegInf = -INFINITY;
@@ -52,8 +53,8 @@ struct AttnKv4Args {
     const std::uint32_t* q_offsets;
     const std::uint32_t* lens;
     unsigned max_queries, max_len;
-    unsigned tiles;                     // row tiles per sequence: ceil(max_queries * group / 8)
-    float scale_log2;                   // scale * log2(e)
+    unsigned tiles;                     // row tiles per sequence: ceil(max_queries * group / ROWS)
+    float scale_log2, q_sign;           // |scale| * log2(e); the scale's sign, 0 for scale 0
     unsigned window, sinks;
     unsigned* counters;                 // [kMaxGrid], zero between calls
     float* part_ml;                     // [2 kMaxGrid][8][2]: reference, sum
@@ -61,15 +62,16 @@ struct AttnKv4Args {
     Kv4View cache;
 };
 
-// One row tile of one sequence: 8 of its (query, head in group) rows.
+// One row tile of one sequence: 4 or 8 of its (query, head in group) rows.
 struct Tile {
     unsigned first_row;   // row of q of the sequence's first query
     unsigned queries, len;
     unsigned flat;        // first flat index query * group + head
-    unsigned rows;        // rows in the tile, 8 at most
+    unsigned rows;        // rows in the tile
     int p_min, p_max;     // positions of its first and last row
     unsigned sinks, low;  // visible: [0, sinks) and [low, p_max]
     unsigned total;       // number of visible keys
+    unsigned clear_from, clear_to;  // of these, the ones that every row sees
 };
 
 template <unsigned D>
@@ -85,9 +87,9 @@ struct Shape {
 template <unsigned D>
 struct Smem {
     alignas(128) unsigned char ring[Shape<D>::ring];  // also the warps' O at a segment's end
-    uint4 q[D / 16][32];                              // A operands: k-step, lane
-    float q_sum[kRows][2];                            // sum of q per group, times scale * log2 e
-    float q_scale[kRows];                             // score per unit of accumulated product
+    alignas(16) __half q[D / 16][32][8];              // operands of QK: k-step, lane (4 halves used by Narrow)
+    float q_sum[kRows][2];                            // sum of the scaled q per group
+    float q_scale[kRows];                             // base-2 score per unit of product with the scaled q
     unsigned valid[kWarps][Shape<D>::stages];         // positions of the step that exist
     float ref[kWarps][kRows], sum[kWarps][kRows], mean[kWarps][kRows][2];
     float row_ref[kRows], row_sum[kRows];
@@ -100,6 +102,28 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, unsigned 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// The first of a chain: c = a b.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint4& a, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
+                                               unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// The 8 x 8 matrix of 16-bit values that lanes hold as row lane / 4, columns 2 (lane % 4), + 1, transposed.
+__device__ __forceinline__ unsigned transpose_f16(unsigned v) {
+    unsigned d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -127,6 +151,7 @@ __device__ __forceinline__ float2 half_unpack(unsigned w) { return __half22float
 
 // The tile `index` of sequence `seq`; total = 0 if it sees nothing, rows = 0
 // if it does not exist. `report`: flag what is out of range.
+template <unsigned ROWS>
 __device__ __forceinline__ Tile make_tile(const AttnKv4Args& a, unsigned seq, unsigned index, bool report) {
     Tile t{};
     t.first_row = a.q_offsets ? __ldg(a.q_offsets + seq) : seq;
@@ -141,9 +166,9 @@ __device__ __forceinline__ Tile make_tile(const AttnKv4Args& a, unsigned seq, un
         if (report) flag_check(B2_CHECK_KV4);
         t.len = 0;
     }
-    t.flat = index * kRows;
+    t.flat = index * ROWS;
     const unsigned all = t.queries * a.group;
-    t.rows = t.flat < all ? min(kRows, all - t.flat) : 0u;
+    t.rows = t.flat < all ? min(ROWS, all - t.flat) : 0u;
     if (t.rows == 0) return t;
     const int base = static_cast<int>(t.len) - static_cast<int>(t.queries);
     t.p_min = base + static_cast<int>(t.flat / a.group);
@@ -153,6 +178,9 @@ __device__ __forceinline__ Tile make_tile(const AttnKv4Args& a, unsigned seq, un
     t.low = low > 0 ? static_cast<unsigned>(low) : 0u;
     t.sinks = min(a.sinks, t.low);
     t.total = t.sinks + static_cast<unsigned>(t.p_max) + 1 - t.low;
+    const int behind = t.p_max - static_cast<int>(a.window) + 1 - static_cast<int>(t.low);
+    t.clear_from = a.window ? t.sinks + (behind > 0 ? static_cast<unsigned>(behind) : 0u) : 0u;
+    t.clear_to = t.p_min < 0 ? 0u : t.sinks + static_cast<unsigned>(t.p_min) + 1 - t.low;
     return t;
 }
 
@@ -177,6 +205,15 @@ __device__ __forceinline__ unsigned lane_page(const AttnKv4Args& a, const Tile& 
     return page;
 }
 
+// Place of 16-byte chunk `part` of key tok's V row in a stage: swizzled inside
+// 128-byte lines, so that the 4 bytes that each of 8 x 4 lanes reads of 4
+// keys' rows hit all banks.
+template <unsigned D>
+__device__ __forceinline__ unsigned v_offset(unsigned tok, unsigned part) {
+    const unsigned line = tok * (D / 2) / 128, at = tok * (D / 2) / 16 % 8 + part;
+    return line * 128 + ((at ^ ((D == 128 ? line & 3u : line & 1u) << 1)) << 4);
+}
+
 // Issues the copies of one step into `stage`; `page` is this lane's.
 template <unsigned D>
 __device__ __forceinline__ void stage_step(const AttnKv4Args& a, const Tile& t, unsigned head, unsigned u0,
@@ -185,36 +222,32 @@ __device__ __forceinline__ void stage_step(const AttnKv4Args& a, const Tile& t, 
     constexpr unsigned PARTS = D / 32;       // 16-byte chunks of a row of codes
     constexpr unsigned COPIES = PARTS;       // chunks per lane
     const unsigned shift = a.cache.page_shift, slots = (1u << shift) - 1u;
-    const unsigned have = __ballot_sync(0xffffffffu, page != kKv4Padding);
-    if (lane == 0) *valid = have;
     const std::uint8_t* heads = a.cache.data + head * a.cache.head_stride;
     const unsigned part = lane % PARTS;
     constexpr unsigned P = 4 * S::groups;
-    // V rows: 16-byte chunks swizzled inside 128-byte lines, so that the 8
-    // bytes (4 at D = 64) that each of 4 x 8 lanes reads hit all banks
-    const auto v_at = [&](unsigned tok) {
-        const unsigned line = tok * (D / 2) / 128, at = tok * (D / 2) / 16 % 8 + part;
-        return stage + S::codes + line * 128 + ((at ^ ((D == 128 ? line & 3u : line & 1u) << 1)) << 4);
-    };
-    const unsigned page0 = __shfl_sync(0xffffffffu, page, 0);
+    // keys lane / PARTS + i * (32 / PARTS): whole swizzle periods apart
+    const unsigned v_at = stage + S::codes + v_offset<D>(lane / PARTS, part);
     const unsigned j0 = key_position(t, u0);
-    if (__all_sync(0xffffffffu, page == page0) && page0 != kKv4Padding &&
-        (u0 >= t.sinks || u0 + kStep <= t.sinks) && ((j0 ^ (j0 + kStep - 1)) >> shift) == 0) {
+    if (u0 + kStep <= t.total && (u0 >= t.sinks || u0 + kStep <= t.sinks) &&
+        ((j0 ^ (j0 + kStep - 1)) >> shift) == 0 && __any_sync(0xffffffffu, page != kKv4Padding)) {
         // 32 neighbours of one page: four runs of memory
-        const std::uint8_t* block = heads + page0 * a.cache.page_stride;
+        if (lane == 0) *valid = 0xFFFFFFFFu;
+        const std::uint8_t* block = heads + page * a.cache.page_stride;
         const unsigned slot = j0 & slots;
         const std::uint8_t* codes = block + (slot * (D / 2) + lane * 16);
         const std::uint8_t* v_codes = codes + kv4_v_codes<D>(shift);
 #pragma unroll
         for (unsigned i = 0; i < COPIES; ++i) {
             copy_async<16>(stage + lane * 16 + i * 512, codes + i * 512, true);
-            copy_async<16>(v_at(i * (32 / PARTS) + lane / PARTS), v_codes + i * 512, true);
+            copy_async<16>(v_at + i * 512, v_codes + i * 512, true);
         }
         const std::uint8_t* params = block + kv4_k_params<D>(shift) + (slot + lane) * P;
         copy_async<P>(stage + 2 * S::codes + lane * P, params, true);
         copy_async<P>(stage + 2 * S::codes + S::params + lane * P, params + (P << shift), true);
         return;
     }
+    const unsigned have = __ballot_sync(0xffffffffu, page != kKv4Padding);
+    if (lane == 0) *valid = have;
 #pragma unroll
     for (unsigned i = 0; i < COPIES; ++i) {
         const unsigned tok = i * (32 / PARTS) + lane / PARTS;
@@ -224,7 +257,7 @@ __device__ __forceinline__ void stage_step(const AttnKv4Args& a, const Tile& t, 
         const std::uint8_t* src =
             ok ? heads + pg * a.cache.page_stride + (slot * (D / 2) + part * 16) : a.cache.data;
         copy_async<16>(stage + tok * (D / 2) + part * 16, src, ok);
-        copy_async<16>(v_at(tok), ok ? src + kv4_v_codes<D>(shift) : src, ok);
+        copy_async<16>(v_at + i * 512, ok ? src + kv4_v_codes<D>(shift) : src, ok);
     }
     const bool ok = page != kKv4Padding;
     const unsigned slot = key_position(t, u0 + lane) & slots;
@@ -246,30 +279,27 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ f32x2 both(float v) { return f2_pack(v, v); }
 
-// What a warp carries through its steps. Thread (r = lane / 4, c = lane % 4)
-// holds row r's reference and its part of the row's sums (even and odd keys),
-// and O^T for rows 2c and 2c + 1, dimensions g * 64 + r * 8 + ...: o[g][n][0]
-// is dimension n of the octet, o[g][n][1] dimension 4 + n.
-template <unsigned D>
-struct WarpState {
-    float ref;
-    f32x2 sum, mean[Shape<D>::groups];
-    f32x2 o[Shape<D>::groups][4][2];
-};
-
+// (w & mask) | bits in one instruction.
+__device__ __forceinline__ unsigned mask_or(unsigned w, unsigned mask, unsigned bits) {
+    unsigned d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(bits));
+    return d;
+}
 // c - 8 of the low (SHIFTED: second) nibbles of both halves of w, in fp16.
 template <bool SHIFTED>
 __device__ __forceinline__ unsigned codes_f16(unsigned w) {
     unsigned d;
-    if (SHIFTED) {  // (1024 + 16 c) / 16 - 72
-        const unsigned x = (w & 0x00F000F0u) | 0x64006400u;
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0x2C002C00u), "r"(0xD480D480u));
-    } else {  // (1024 + c) - 1032
-        const unsigned x = (w & 0x000F000Fu) | 0x64006400u;
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0xE408E408u));
-    }
+    if (SHIFTED)  // (1024 + 16 c) / 16 - 72
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(mask_or(w, 0x00F000F0u, 0x64006400u)), "r"(0x2C002C00u), "r"(0xD480D480u));
+    else  // (1024 + c) - 1032
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(mask_or(w, 0x000F000Fu, 0x64006400u)), "r"(0xE408E408u));
     return d;
 }
 
@@ -287,198 +317,586 @@ __device__ __forceinline__ bool nonfinite_params(unsigned w) {
     return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
 }
 
-// One step of 32 keys. MASKED: some row does not see some of them.
-template <unsigned D, bool MASKED>
-__device__ __forceinline__ void attend_step(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned stage,
-                                            unsigned u0, unsigned valid, int pos, float q_scale,
-                                            const float (&q_sum)[Shape<D>::groups], unsigned lane,
-                                            WarpState<D>& st) {
-    using S = Shape<D>;
-    constexpr unsigned G = S::groups;
-    const unsigned r = lane / 4, c = lane % 4;
+// Columns first, first + 1 of a thread's O^T as rows of 128-bit stores.
+template <unsigned PITCH, unsigned D>
+__device__ __forceinline__ void put_columns(const f32x2 (&o)[Shape<D>::groups][4][2], float* warp_o, unsigned first,
+                                            unsigned rows, unsigned r) {
+#pragma unroll
+    for (unsigned e = 0; e < 2; ++e)
+        if (first + e < rows) {
+            float* row = warp_o + (first + e) * PITCH + r * 8;
+#pragma unroll
+            for (unsigned g = 0; g < Shape<D>::groups; ++g) {
+                float v[8];
+#pragma unroll
+                for (unsigned n = 0; n < 4; ++n) {
+                    const float2 y0 = f2_unpack(o[g][n][0]), y1 = f2_unpack(o[g][n][1]);
+                    v[n] = e ? y0.y : y0.x;
+                    v[4 + n] = e ? y1.y : y1.x;
+                }
+                *reinterpret_cast<float4*>(row + g * 64) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(row + g * 64 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        }
+}
 
-    // ---- scores: x[b] holds keys 8b + 2c and 8b + 2c + 1 of row r ----
-    f32x2 x[4] = {0, 0, 0, 0};
-    {
-        unsigned kw[4][2 * G], kp[4][2 * G];
+// Position of the tile's row r; -1 past its rows.
+__device__ __forceinline__ int row_position(const AttnKv4Args& a, const Tile& t, unsigned r) {
+    return r < t.rows ? static_cast<int>(t.len) - static_cast<int>(t.queries) + static_cast<int>((t.flat + r) / a.group)
+                      : -1;
+}
+
+// ---- a warp's steps ----------------------------------------------------------------
+//
+// Both kinds hold, for a step of 32 keys, the scores in fp32, p and p s, and
+// O^T as accumulators of M = 16 dimensions x N = 8 columns: thread (r = lane /
+// 4, c = lane % 4) has columns 2c and 2c + 1 of dimensions g * 64 + r * 8 +
+// n (o[g][n][0]) and + 4 + n (o[g][n][1]), n < 4. Sums are parts that the
+// end adds up: ps = sum p s, mean = sum p m per group.
+
+// The affine part of the scores, s (8 sum q) + m (sum q), is one product: the
+// parameter words are (s, m) pairs in bf16 as they lie. (8 sum q, sum q) of
+// group c % G in three bf16 parts: parts c / G (k = 2c) and 2 (k = 2c + 8).
+template <unsigned G>
+__device__ __forceinline__ void affine_operand(float q_sum, unsigned c, unsigned (&operand)[2]) {
+    float a8 = 8.0f * q_sum, a1 = q_sum;
+    unsigned p[3];
+#pragma unroll
+    for (unsigned i = 0; i < 3; ++i) {
+        p[i] = bf16_pack(a8, a1);
+        a8 -= bf16_low(p[i]);
+        a1 -= bf16_high(p[i]);
+    }
+    operand[0] = c < G ? p[0] : c < 2 * G ? p[1] : 0u;
+    operand[1] = c < G ? p[2] : 0u;
+}
+
+// s < 2^(exponent - 126) for the largest s; the reference that puts p s of
+// score `top` (scaled) into [2^10, 2^11).
+__device__ __forceinline__ float reference_for(float top, float q_scale, unsigned exponent) {
+    return fmaf(top, q_scale, static_cast<float>(max(static_cast<int>(exponent) - 137, -71)));
+}
+
+__device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, unsigned tok, int j, int pos) {
+    return ((valid >> tok) & 1u) && j <= pos &&
+           (a.window == 0 || pos - j < static_cast<int>(a.window) || j < static_cast<int>(a.sinks));
+}
+
+// Eight rows. Queries are the M = 16 operand of QK (hi parts in rows 0..7, lo
+// in 8..15), so thread (r, c) gets the scores of row r and keys 8b + 2c, + 1,
+// which is where the second product wants P^T (k = keys, n = rows).
+template <unsigned D>
+struct Wide {
+    static constexpr unsigned ROWS = 8, G = Shape<D>::groups;
+    using S = Shape<D>;
+    unsigned lane, r, c, affine[2];
+    float q_scale;
+    int pos;
+    float ref;
+    f32x2 sum, mean[G], ps[G];
+    f32x2 o[G][4][2];
+
+    __device__ __forceinline__ void init(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned lane_) {
+        lane = lane_;
+        r = lane / 4;
+        c = lane % 4;
+        q_scale = sm.q_scale[r];
+        affine_operand<G>(sm.q_sum[r][c % G], c, affine);
+        pos = row_position(a, t, r);
+        ref = kNegInf;
+        sum = 0;
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) {
+            mean[g] = ps[g] = 0;
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) o[g][n][0] = o[g][n][1] = 0;
+        }
+    }
+    // Half `half` of pair (i, i + 4), i = 2 * (k-step % 2) + reg, of row `row`.
+    static __device__ __forceinline__ void put_query(Smem<D>& sm, unsigned row, unsigned step, unsigned c, unsigned reg,
+                                                     unsigned half, __half hi, __half lo) {
+        __half* at = sm.q[step][row * 4 + c] + reg * 4 + half;
+        at[0] = hi;
+        at[2] = lo;
+    }
+
+    // MASKED: some row does not see some of the keys.
+    template <bool MASKED>
+    __device__ __forceinline__ void step(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned stage,
+                                         unsigned u0, unsigned valid) {
+        // ---- scores: x[b] holds keys 8b + 2c and 8b + 2c + 1 of row r ----
+        f32x2 x[4];
+        {
+#pragma unroll
+            for (unsigned b = 0; b < 4; ++b) {
+                unsigned w;
+                lds_n<1>(stage + 2 * S::codes + (8 * b + r) * 4 * G + c % G * 4, &w);
+                float y[4];
+                mma_bf16_first(y, affine[0], 0u, affine[1], 0u, w, w);
+                x[b] = f2_pack(y[0], y[1]);
+            }
+            unsigned kw[4][2 * G], kp[4][2 * G];
+#pragma unroll
+            for (unsigned b = 0; b < 4; ++b) {
+                lds_n<2 * G>(stage + (8 * b + r) * (D / 2) + c * (D / 8), kw[b]);
+                lds_n<2 * G>(stage + 2 * S::codes + (8 * b + 2 * c) * 4 * G, kp[b]);
+            }
+#pragma unroll
+            for (unsigned g = 0; g < G; ++g) {
+                float acc[4][4];
+#pragma unroll
+                for (unsigned k = 0; k < 4; ++k) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(sm.q[g * 4 + k][lane]);
+#pragma unroll
+                    for (unsigned b = 0; b < 4; ++b) {
+                        const unsigned w = kw[b][g * 2 + k / 2] >> (k % 2 * 8);
+                        if (k == 0) mma_f16_first(acc[b], q, codes_f16<false>(w), codes_f16<true>(w));
+                        else mma_f16(acc[b], q, codes_f16<false>(w), codes_f16<true>(w));
+                    }
+                }
+#pragma unroll
+                for (unsigned b = 0; b < 4; ++b) {
+                    const f32x2 dot = add2(f2_pack(acc[b][0], acc[b][1]), f2_pack(acc[b][2], acc[b][3]));
+                    x[b] = f2_fma(f2_pack(bf16_low(kp[b][g]), bf16_low(kp[b][G + g])), dot, x[b]);
+                }
+            }
+        }
+        unsigned vp[4][2 * G];
+#pragma unroll
+        for (unsigned b = 0; b < 4; ++b) lds_n<2 * G>(stage + 2 * S::codes + S::params + (8 * b + 2 * c) * 4 * G, vp[b]);
+        if (MASKED) {
+#pragma unroll
+            for (unsigned b = 0; b < 4; ++b) {
+                float2 y = f2_unpack(x[b]);
+#pragma unroll
+                for (unsigned e = 0; e < 2; ++e) {
+                    const unsigned tok = 8 * b + 2 * c + e;
+                    const int j = static_cast<int>(key_position(t, u0 + tok));
+                    const bool seen = visible(a, valid, tok, j, pos);
+                    if (!seen) (e ? y.y : y.x) = kNegInf;
+                    // a value that is not finite reaches the rows that see it
+                    // (through the mean's sum), and not the others (0 * NaN)
+#pragma unroll
+                    for (unsigned g = 0; g < G; ++g) {
+                        unsigned& w = vp[b][e * G + g];
+                        if (nonfinite_params(w)) {
+                            w = 0;
+                            if (seen) mean[g] = both(NAN);
+                        }
+                    }
+                }
+                x[b] = f2_pack(y.x, y.y);
+            }
+        }
+
+        // ---- the reference: p s is to stay below 2^15 ----
+        // A thread packs p s of its own keys only, so each tests its own; what has
+        // to be exchanged is exchanged when some reference has to rise.
+        float top = kNegInf;
+        unsigned top_w = vp[0][0];  // maxima of both halves of the words: s is the lower
 #pragma unroll
         for (unsigned b = 0; b < 4; ++b) {
-            lds_n<2 * G>(stage + (8 * b + r) * (D / 2) + c * (D / 8), kw[b]);
-            lds_n<2 * G>(stage + 2 * S::codes + (8 * b + 2 * c) * 4 * G, kp[b]);
+            const float2 y = f2_unpack(x[b]);
+            top = fmaxf(top, fmaxf(y.x, y.y));
+#pragma unroll
+            for (unsigned i = 0; i < 2 * G; ++i) top_w = __vmaxu2(top_w, vp[b][i]);
+        }
+        float need = reference_for(top, q_scale, top_w >> 7 & 0xFFu);
+        if (__any_sync(0xffffffffu, need > ref + 4.0f)) {
+            if ((top_w & 0x7F80u) == 0x7F80u) {  // a step that is not finite has no part in the reference
+                unsigned finite_s = 0;
+#pragma unroll
+                for (unsigned b = 0; b < 4; ++b)
+#pragma unroll
+                    for (unsigned i = 0; i < 2 * G; ++i)
+                        if ((vp[b][i] & 0x7F80u) != 0x7F80u) finite_s = max(finite_s, vp[b][i] & 0x7F80u);
+                need = reference_for(top, q_scale, finite_s >> 7);
+            }
+            need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 1));
+            need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 2));
+            const float next = need > ref + 4.0f ? need : ref;
+            const float alpha = next == ref ? 1.0f : exp2_approx(ref - next);
+            ref = next;
+            sum = mul2(sum, both(alpha));
+            const f32x2 cols = f2_pack(__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4));
+#pragma unroll
+            for (unsigned g = 0; g < G; ++g) {
+                mean[g] = mul2(mean[g], both(alpha));
+                ps[g] = mul2(ps[g], both(alpha));
+#pragma unroll
+                for (unsigned n = 0; n < 4; ++n) {
+                    o[g][n][0] = mul2(o[g][n][0], cols);
+                    o[g][n][1] = mul2(o[g][n][1], cols);
+                }
+            }
+        }
+        const float at = ref == kNegInf ? 0.0f : ref;
+        f32x2 steps[G][4];
+#pragma unroll
+        for (unsigned b = 0; b < 4; ++b) {
+            const float2 y = f2_unpack(f2_fma(x[b], both(q_scale), both(-at)));
+            x[b] = f2_pack(exp2_approx(y.x), exp2_approx(y.y));
+            sum = add2(sum, x[b]);
+#pragma unroll
+            for (unsigned g = 0; g < G; ++g) {
+                steps[g][b] = f2_pack(bf16_low(vp[b][g]), bf16_low(vp[b][G + g]));
+                mean[g] = f2_fma(x[b], f2_pack(bf16_high(vp[b][g]), bf16_high(vp[b][G + g])), mean[g]);
+            }
+        }
+
+        // ---- O^T += V^T (p s)^T ----
+        const unsigned v_base = stage + S::codes + v_offset<D>(2 * c, r * G * 4 / 16) + r * G * 4 % 16;
+        const unsigned v_next = stage + S::codes + v_offset<D>(2 * c + 1, r * G * 4 / 16) + r * G * 4 % 16;
+        unsigned vw[8][G];  // the lane's octets of keys 8b + 2c and 8b + 2c + 1
+#pragma unroll
+        for (unsigned b = 0; b < 4; ++b) {
+            lds_n<G>(v_base + 8 * b * (D / 2), vw[2 * b]);
+            lds_n<G>(v_next + 8 * b * (D / 2), vw[2 * b + 1]);
         }
 #pragma unroll
         for (unsigned g = 0; g < G; ++g) {
-            float acc[4][4];
-#pragma unroll
-            for (unsigned b = 0; b < 4; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.0f;
-#pragma unroll
-            for (unsigned k = 0; k < 4; ++k) {
-                const uint4 q = sm.q[g * 4 + k][lane];
-#pragma unroll
-                for (unsigned b = 0; b < 4; ++b) {
-                    const unsigned w = kw[b][g * 2 + k / 2] >> (k % 2 * 8);
-                    mma_f16(acc[b], q, codes_f16<false>(w), codes_f16<true>(w));
-                }
-            }
+            unsigned hi[4], lo[4], xa[4], ya[4];
 #pragma unroll
             for (unsigned b = 0; b < 4; ++b) {
-                const f32x2 dot = add2(f2_pack(acc[b][0], acc[b][1]), f2_pack(acc[b][2], acc[b][3]));
-                const f32x2 step = f2_pack(bf16_low(kp[b][g]), bf16_low(kp[b][G + g]));
-                const f32x2 mid = f2_fma(step, both(8.0f), f2_pack(bf16_high(kp[b][g]), bf16_high(kp[b][G + g])));
-                x[b] = f2_fma(mul2(step, dot), both(q_scale), x[b]);
-                x[b] = f2_fma(mid, both(q_sum[g]), x[b]);
+                const unsigned w0 = vw[2 * b][g], w1 = vw[2 * b + 1][g];
+                const f32x2 v = mul2(x[b], steps[g][b]);
+                const float2 y = f2_unpack(v);
+                ps[g] = add2(ps[g], v);
+                hi[b] = half_pack(y.x, y.y);
+                const float2 h = half_unpack(hi[b]);
+                const float2 rest = f2_unpack(sub2(v, f2_pack(h.x, h.y)));
+                lo[b] = half_pack(rest.x, rest.y);
+                xa[b] = __byte_perm(w0, w1, 0x5410);
+                ya[b] = __byte_perm(w0, w1, 0x7632);
+            }
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) {
+                const unsigned sh = n / 2 * 8;
+                float acc[4];
+#pragma unroll
+                for (unsigned h = 0; h < 2; ++h) {
+                    const unsigned w[4] = {xa[2 * h] >> sh, ya[2 * h] >> sh, xa[2 * h + 1] >> sh, ya[2 * h + 1] >> sh};
+                    const uint4 v = n % 2 ? make_uint4(codes_f16<true>(w[0]), codes_f16<true>(w[1]), codes_f16<true>(w[2]),
+                                                       codes_f16<true>(w[3]))
+                                          : make_uint4(codes_f16<false>(w[0]), codes_f16<false>(w[1]),
+                                                       codes_f16<false>(w[2]), codes_f16<false>(w[3]));
+                    if (h == 0) mma_f16_first(acc, v, hi[0], hi[1]);
+                    else mma_f16(acc, v, hi[2], hi[3]);
+                    mma_f16(acc, v, lo[2 * h], lo[2 * h + 1]);
+                }
+                o[g][n][0] = add2(o[g][n][0], f2_pack(acc[0], acc[1]));
+                o[g][n][1] = add2(o[g][n][1], f2_pack(acc[2], acc[3]));
             }
         }
     }
-    unsigned vp[4][2 * G];
+
+    // The warp's sums into shared memory: references, sums and means now, O
+    // (row pitch PITCH) once the rings are drained.
+    __device__ __forceinline__ void put_sums(Smem<D>& sm, unsigned warp) {
+        const auto total = [](f32x2 v) {
+            const float2 y = f2_unpack(v);
+            float x = y.x + y.y;
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            return x + __shfl_xor_sync(0xffffffffu, x, 2);
+        };
+        const float l = total(sum);
+        float m[G];
 #pragma unroll
-    for (unsigned b = 0; b < 4; ++b) lds_n<2 * G>(stage + 2 * S::codes + S::params + (8 * b + 2 * c) * 4 * G, vp[b]);
-    if (MASKED) {
+        for (unsigned g = 0; g < G; ++g) m[g] = fmaf(8.0f, total(ps[g]), total(mean[g]));
+        if (c == 0) {
+            sm.ref[warp][r] = ref;
+            sm.sum[warp][r] = l;
 #pragma unroll
-        for (unsigned b = 0; b < 4; ++b) {
-            float2 y = f2_unpack(x[b]);
+            for (unsigned g = 0; g < G; ++g) sm.mean[warp][r][g] = m[g];
+        }
+    }
+    template <unsigned PITCH>
+    __device__ __forceinline__ void put_o(float* warp_o, unsigned rows) {
+        put_columns<PITCH, D>(o, warp_o, 2 * c, rows, r);
+    }
+};
+
+// Four rows (one token of a group of four heads): with eight columns each
+// matrix instruction would be half empty, and these instructions are what a
+// step costs most, so hi and lo parts share the columns: 34 of them instead
+// of 68. Keys are the M = 16 operand of QK; columns n < 4 are the rows' hi
+// parts, n >= 4 their lo parts, and the lanes of the two halves exchange, so
+// that a thread ends with rows 2 (c & 1), + 1 of two keys: 16 (c >= 2) + 8 h +
+// r. P s is split into hi and lo again, exchanged, and transposed by
+// movmatrix into the operand of the second product.
+template <unsigned D>
+struct Narrow {
+    static constexpr unsigned ROWS = 4, G = Shape<D>::groups;
+    using S = Shape<D>;
+    unsigned lane, r, c, affine[2];
+    unsigned q[D / 16][2];
+    f32x2 q_scale;
+    int pos[2];
+    f32x2 ref, sum, mean[G], ps[G];
+    f32x2 o[G][4][2];
+
+    __device__ __forceinline__ void init(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned lane_) {
+        lane = lane_;
+        r = lane / 4;
+        c = lane % 4;
+        const unsigned row = 2 * (c & 1u);
+        q_scale = f2_pack(sm.q_scale[row], sm.q_scale[row + 1]);
+        affine_operand<G>(r < ROWS ? sm.q_sum[r][c % G] : 0.0f, c, affine);
+        pos[0] = row_position(a, t, row);
+        pos[1] = row_position(a, t, row + 1);
 #pragma unroll
-            for (unsigned e = 0; e < 2; ++e) {
-                const unsigned tok = 8 * b + 2 * c + e;
+        for (unsigned k = 0; k < D / 16; ++k) {
+            const uint2 v = *reinterpret_cast<const uint2*>(sm.q[k][lane]);
+            q[k][0] = v.x;
+            q[k][1] = v.y;
+        }
+        ref = both(kNegInf);
+        sum = 0;
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) {
+            mean[g] = ps[g] = 0;
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) o[g][n][0] = o[g][n][1] = 0;
+        }
+    }
+    static __device__ __forceinline__ void put_query(Smem<D>& sm, unsigned row, unsigned step, unsigned c, unsigned reg,
+                                                     unsigned half, __half hi, __half lo) {
+        sm.q[step][row * 4 + c][reg * 2 + half] = hi;
+        sm.q[step][(row + ROWS) * 4 + c][reg * 2 + half] = lo;
+    }
+
+    template <bool MASKED>
+    __device__ __forceinline__ void step(const AttnKv4Args& a, const Tile& t, const Smem<D>&, unsigned stage, unsigned u0,
+                                         unsigned valid) {
+        const bool upper = c & 2u;
+        // ---- scores: y[k][h] is key 16k + 8h + r, columns 2c and 2c + 1 ----
+        f32x2 y[2][2];
+#pragma unroll
+        for (unsigned k = 0; k < 2; ++k) {
+            const unsigned tok = 16 * k + r, codes = stage + tok * (D / 2) + c * (D / 8);
+            unsigned w0[2 * G], w1[2 * G], p0[G], p1[G];
+            lds_n<2 * G>(codes, w0);
+            lds_n<2 * G>(codes + 8 * (D / 2), w1);
+            lds_n<G>(stage + 2 * S::codes + tok * 4 * G, p0);
+            lds_n<G>(stage + 2 * S::codes + (tok + 8) * 4 * G, p1);
+            {
+                const unsigned a0 = G == 1 || !(c & 1u) ? p0[0] : p0[G - 1], a1 = G == 1 || !(c & 1u) ? p1[0] : p1[G - 1];
+                float acc[4];
+                mma_bf16_first(acc, a0, a1, a0, a1, affine[0], affine[1]);
+                y[k][0] = f2_pack(acc[0], acc[1]);
+                y[k][1] = f2_pack(acc[2], acc[3]);
+            }
+#pragma unroll
+            for (unsigned g = 0; g < G; ++g) {
+                float acc[4];
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) {
+                    const unsigned x0 = w0[g * 2 + i / 2] >> (i % 2 * 8), x1 = w1[g * 2 + i / 2] >> (i % 2 * 8);
+                    const uint4 v = make_uint4(codes_f16<false>(x0), codes_f16<false>(x1), codes_f16<true>(x0),
+                                               codes_f16<true>(x1));
+                    if (i == 0) mma_f16_first(acc, v, q[g * 4][0], q[g * 4][1]);
+                    else mma_f16(acc, v, q[g * 4 + i][0], q[g * 4 + i][1]);
+                }
+                y[k][0] = f2_fma(both(bf16_low(p0[g])), f2_pack(acc[0], acc[1]), y[k][0]);
+                y[k][1] = f2_fma(both(bf16_low(p1[g])), f2_pack(acc[2], acc[3]), y[k][1]);
+            }
+        }
+        // hi + lo: the lower lanes keep keys 0..15, the upper ones 16..31
+        f32x2 x[2];
+        unsigned vp[2][G];
+        const unsigned first = (upper ? 16u : 0u) + r;
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            const float2 give = f2_unpack(upper ? y[0][h] : y[1][h]);
+            x[h] = add2(upper ? y[1][h] : y[0][h], f2_pack(__shfl_xor_sync(0xffffffffu, give.x, 2),
+                                                           __shfl_xor_sync(0xffffffffu, give.y, 2)));
+            lds_n<G>(stage + 2 * S::codes + S::params + (first + 8 * h) * 4 * G, vp[h]);
+        }
+        if (MASKED) {
+#pragma unroll
+            for (unsigned h = 0; h < 2; ++h) {
+                const unsigned tok = first + 8 * h;
                 const int j = static_cast<int>(key_position(t, u0 + tok));
-                const bool seen = ((valid >> tok) & 1u) && j <= pos &&
-                                  (a.window == 0 || pos - j < static_cast<int>(a.window) || j < static_cast<int>(a.sinks));
-                if (!seen) (e ? y.y : y.x) = kNegInf;
+                const bool seen0 = visible(a, valid, tok, j, pos[0]), seen1 = visible(a, valid, tok, j, pos[1]);
+                const float2 v = f2_unpack(x[h]);
+                x[h] = f2_pack(seen0 ? v.x : kNegInf, seen1 ? v.y : kNegInf);
                 // a value that is not finite reaches the rows that see it
                 // (through the mean's sum), and not the others (0 * NaN)
 #pragma unroll
+                for (unsigned g = 0; g < G; ++g)
+                    if (nonfinite_params(vp[h][g])) {
+                        vp[h][g] = 0;
+                        mean[g] = add2(mean[g], f2_pack(seen0 ? NAN : 0.0f, seen1 ? NAN : 0.0f));
+                    }
+            }
+        }
+
+        // ---- the references: p s is to stay below 2^15 ----
+        // A thread packs p s of its own keys only, so each tests its own; what
+        // has to be exchanged is exchanged when some reference has to rise.
+        {
+            const float2 x0 = f2_unpack(x[0]), x1 = f2_unpack(x[1]), scale = f2_unpack(q_scale), old = f2_unpack(ref);
+            const float top0 = fmaxf(x0.x, x1.x), top1 = fmaxf(x0.y, x1.y);
+            unsigned top_w = __vmaxu2(vp[0][0], vp[1][0]);  // maxima of both halves: s is the lower
+            if (G == 2) top_w = __vmaxu2(top_w, __vmaxu2(vp[0][G - 1], vp[1][G - 1]));
+            const unsigned exponent = top_w >> 7 & 0xFFu;
+            float need0 = reference_for(top0, scale.x, exponent), need1 = reference_for(top1, scale.y, exponent);
+            if (__any_sync(0xffffffffu, need0 > old.x + 4.0f || need1 > old.y + 4.0f)) {
+                if (exponent == 0xFFu) {  // a step that is not finite has no part in the reference
+                    unsigned finite_s = 0;
+#pragma unroll
+                    for (unsigned h = 0; h < 2; ++h)
+#pragma unroll
+                        for (unsigned g = 0; g < G; ++g)
+                            if ((vp[h][g] & 0x7F80u) != 0x7F80u) finite_s = max(finite_s, vp[h][g] & 0x7F80u);
+                    need0 = reference_for(top0, scale.x, finite_s >> 7);
+                    need1 = reference_for(top1, scale.y, finite_s >> 7);
+                }
+#pragma unroll
+                for (unsigned i = 2; i < 32; i *= 2) {
+                    need0 = fmaxf(need0, __shfl_xor_sync(0xffffffffu, need0, i));
+                    need1 = fmaxf(need1, __shfl_xor_sync(0xffffffffu, need1, i));
+                }
+                const float ref0 = need0 > old.x + 4.0f ? need0 : old.x, ref1 = need1 > old.y + 4.0f ? need1 : old.y;
+                const f32x2 alpha = f2_pack(ref0 == old.x ? 1.0f : exp2_approx(old.x - ref0),
+                                            ref1 == old.y ? 1.0f : exp2_approx(old.y - ref1));
+                ref = f2_pack(ref0, ref1);
+                sum = mul2(sum, alpha);
+#pragma unroll
                 for (unsigned g = 0; g < G; ++g) {
-                    unsigned& w = vp[b][e * G + g];
-                    if (nonfinite_params(w)) {
-                        w = 0;
-                        if (seen) st.mean[g] = both(NAN);
+                    mean[g] = mul2(mean[g], alpha);
+                    ps[g] = mul2(ps[g], alpha);
+#pragma unroll
+                    for (unsigned n = 0; n < 4; ++n) {
+                        o[g][n][0] = mul2(o[g][n][0], alpha);
+                        o[g][n][1] = mul2(o[g][n][1], alpha);
                     }
                 }
             }
-            x[b] = f2_pack(y.x, y.y);
         }
-    }
-
-    // ---- the reference: p s is to stay below 2^15 ----
-    unsigned top_s = 0;
-#pragma unroll
-    for (unsigned b = 0; b < 4; ++b)
-#pragma unroll
-        for (unsigned i = 0; i < 2 * G; ++i) top_s = max(top_s, vp[b][i] << 16);
-    top_s = __reduce_max_sync(0xffffffffu, top_s);
-    if (top_s >= 0x7F800000u) {  // a step that is not finite has no part in the reference
-        top_s = 0;
-#pragma unroll
-        for (unsigned b = 0; b < 4; ++b)
-#pragma unroll
-            for (unsigned i = 0; i < 2 * G; ++i)
-                if ((vp[b][i] << 16) < 0x7F800000u) top_s = max(top_s, vp[b][i] << 16);
-        top_s = __reduce_max_sync(0xffffffffu, top_s);
-    }
-    const float s_log2 = static_cast<float>(max(static_cast<int>(top_s >> 23) - 126, -60));
-    float top = kNegInf;
-#pragma unroll
-    for (unsigned b = 0; b < 4; ++b) {
-        const float2 y = f2_unpack(x[b]);
-        top = fmaxf(top, fmaxf(y.x, y.y));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float need = top + s_log2 - 11.0f;
-    const bool raise = need > st.ref + 4.0f;
-    if (__any_sync(0xffffffffu, raise)) {
-        const float ref = raise ? need : st.ref;
-        const float alpha = raise ? exp2_approx(st.ref - ref) : 1.0f;
-        st.ref = ref;
-        st.sum = mul2(st.sum, both(alpha));
-        const f32x2 cols = f2_pack(__shfl_sync(0xffffffffu, alpha, 8 * c), __shfl_sync(0xffffffffu, alpha, 8 * c + 4));
-#pragma unroll
-        for (unsigned g = 0; g < G; ++g) {
-            st.mean[g] = mul2(st.mean[g], both(alpha));
-#pragma unroll
-            for (unsigned n = 0; n < 4; ++n) {
-                st.o[g][n][0] = mul2(st.o[g][n][0], cols);
-                st.o[g][n][1] = mul2(st.o[g][n][1], cols);
-            }
-        }
-    }
-    const float ref = st.ref == kNegInf ? 0.0f : st.ref;
-    f32x2 steps[G][4];
-#pragma unroll
-    for (unsigned b = 0; b < 4; ++b) {
-        const float2 y = f2_unpack(add2(x[b], both(-ref)));
-        x[b] = f2_pack(exp2_approx(y.x), exp2_approx(y.y));
-        st.sum = add2(st.sum, x[b]);
-#pragma unroll
-        for (unsigned g = 0; g < G; ++g) {
-            steps[g][b] = f2_pack(bf16_low(vp[b][g]), bf16_low(vp[b][G + g]));
-            const f32x2 mid =
-                f2_fma(steps[g][b], both(8.0f), f2_pack(bf16_high(vp[b][g]), bf16_high(vp[b][G + g])));
-            st.mean[g] = f2_fma(x[b], mid, st.mean[g]);
-        }
-    }
-
-    // ---- O^T += V^T (p s)^T ----
-    unsigned vw[8][G];
-#pragma unroll
-    for (unsigned b = 0; b < 4; ++b)
-#pragma unroll
-        for (unsigned e = 0; e < 2; ++e) {
-            const unsigned tok = 8 * b + 2 * c + e;
-            const unsigned line = tok * (D / 2) / 128, at = tok * (D / 2) / 16 % 8 + r * G * 4 / 16;
-            const unsigned sw = at ^ ((D == 128 ? line & 3u : line & 1u) << 1);
-            lds_n<G>(stage + S::codes + line * 128 + sw * 16 + (r * G * 4) % 16, vw[2 * b + e]);
-        }
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-        unsigned hi[4], lo[4], xa[4], ya[4];
-#pragma unroll
-        for (unsigned b = 0; b < 4; ++b) {
-            const f32x2 ps = mul2(x[b], steps[g][b]);
-            const float2 y = f2_unpack(ps);
-            hi[b] = half_pack(y.x, y.y);
-            const float2 h = half_unpack(hi[b]);
-            const float2 rest = f2_unpack(f2_fma(f2_pack(h.x, h.y), both(-1.0f), ps));
-            lo[b] = half_pack(rest.x, rest.y);
-            xa[b] = __byte_perm(vw[2 * b][g], vw[2 * b + 1][g], 0x5410);
-            ya[b] = __byte_perm(vw[2 * b][g], vw[2 * b + 1][g], 0x7632);
-        }
-#pragma unroll
-        for (unsigned n = 0; n < 4; ++n) {
-            const unsigned sh = n / 2 * 8;
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        {
+            const float2 at = f2_unpack(ref);
+            const f32x2 minus = f2_pack(at.x == kNegInf ? 0.0f : -at.x, at.y == kNegInf ? 0.0f : -at.y);
 #pragma unroll
             for (unsigned h = 0; h < 2; ++h) {
-                const unsigned w[4] = {xa[2 * h] >> sh, ya[2 * h] >> sh, xa[2 * h + 1] >> sh, ya[2 * h + 1] >> sh};
-                const uint4 v = n % 2 ? make_uint4(codes_f16<true>(w[0]), codes_f16<true>(w[1]), codes_f16<true>(w[2]),
-                                                   codes_f16<true>(w[3]))
-                                      : make_uint4(codes_f16<false>(w[0]), codes_f16<false>(w[1]),
-                                                   codes_f16<false>(w[2]), codes_f16<false>(w[3]));
-                mma_f16(acc, v, hi[2 * h], hi[2 * h + 1]);
-                mma_f16(acc, v, lo[2 * h], lo[2 * h + 1]);
+                const float2 v = f2_unpack(f2_fma(x[h], q_scale, minus));
+                x[h] = f2_pack(exp2_approx(v.x), exp2_approx(v.y));
+                sum = add2(sum, x[h]);
             }
-            st.o[g][n][0] = add2(st.o[g][n][0], f2_pack(acc[0], acc[1]));
-            st.o[g][n][1] = add2(st.o[g][n][1], f2_pack(acc[2], acc[3]));
+        }
+
+        // ---- O^T += V^T (p s)^T ----
+        const unsigned v_base = stage + S::codes + v_offset<D>(2 * c, r * G * 4 / 16) + r * G * 4 % 16;
+        const unsigned v_next = stage + S::codes + v_offset<D>(2 * c + 1, r * G * 4 / 16) + r * G * 4 % 16;
+        unsigned vw[8][G];  // the lane's octets of keys 8b + 2c and 8b + 2c + 1
+#pragma unroll
+        for (unsigned b = 0; b < 4; ++b) {
+            lds_n<G>(v_base + 8 * b * (D / 2), vw[2 * b]);
+            lds_n<G>(v_next + 8 * b * (D / 2), vw[2 * b + 1]);
+        }
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) {
+            unsigned b[2][2];  // keys 16k + 8h + 2c, + 1 of column r
+#pragma unroll
+            for (unsigned h = 0; h < 2; ++h) {
+                const f32x2 v = mul2(x[h], both(bf16_low(vp[h][g])));
+                mean[g] = f2_fma(x[h], both(bf16_high(vp[h][g])), mean[g]);
+                ps[g] = add2(ps[g], v);
+                const float2 f = f2_unpack(v);
+                const unsigned hi = half_pack(f.x, f.y);
+                const float2 up = half_unpack(hi);
+                const float2 rest = f2_unpack(sub2(v, f2_pack(up.x, up.y)));
+                const unsigned lo = half_pack(rest.x, rest.y);
+                const unsigned got = __shfl_xor_sync(0xffffffffu, upper ? hi : lo, 2);
+                b[0][h] = transpose_f16(upper ? got : hi);
+                b[1][h] = transpose_f16(upper ? lo : got);
+            }
+            unsigned xa[4], ya[4];
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i) {
+                xa[i] = __byte_perm(vw[2 * i][g], vw[2 * i + 1][g], 0x5410);
+                ya[i] = __byte_perm(vw[2 * i][g], vw[2 * i + 1][g], 0x7632);
+            }
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) {
+                const unsigned sh = n / 2 * 8;
+                float acc[4];
+#pragma unroll
+                for (unsigned k = 0; k < 2; ++k) {
+                    const unsigned w[4] = {xa[2 * k] >> sh, ya[2 * k] >> sh, xa[2 * k + 1] >> sh, ya[2 * k + 1] >> sh};
+                    const uint4 v = n % 2 ? make_uint4(codes_f16<true>(w[0]), codes_f16<true>(w[1]), codes_f16<true>(w[2]),
+                                                       codes_f16<true>(w[3]))
+                                          : make_uint4(codes_f16<false>(w[0]), codes_f16<false>(w[1]),
+                                                       codes_f16<false>(w[2]), codes_f16<false>(w[3]));
+                    if (k == 0) mma_f16_first(acc, v, b[0][0], b[0][1]);
+                    else mma_f16(acc, v, b[1][0], b[1][1]);
+                }
+                o[g][n][0] = add2(o[g][n][0], f2_pack(acc[0], acc[1]));
+                o[g][n][1] = add2(o[g][n][1], f2_pack(acc[2], acc[3]));
+            }
         }
     }
-}
 
-// The tile's queries as A operands: hi parts in rows 0..7, lo parts in 8..15,
-// each row scaled by a power of two to about 2^9 at most.
-template <typename T, unsigned D>
+    __device__ __forceinline__ void put_sums(Smem<D>& sm, unsigned warp) {
+        const auto total = [](f32x2 v) {
+            float2 y = f2_unpack(v);
+#pragma unroll
+            for (unsigned i = 2; i < 32; i *= 2) {
+                y.x += __shfl_xor_sync(0xffffffffu, y.x, i);
+                y.y += __shfl_xor_sync(0xffffffffu, y.y, i);
+            }
+            return y;
+        };
+        const float2 l = total(sum), at = f2_unpack(ref);
+        const unsigned row = 2 * (c & 1u);
+        const bool writes = r == 0 && c < 2;
+        if (writes) {
+            sm.ref[warp][row] = at.x;
+            sm.ref[warp][row + 1] = at.y;
+            sm.sum[warp][row] = l.x;
+            sm.sum[warp][row + 1] = l.y;
+        }
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) {
+            const float2 m = total(mean[g]), s = total(ps[g]);
+            if (writes) {
+                sm.mean[warp][row][g] = fmaf(8.0f, s.x, m.x);
+                sm.mean[warp][row + 1][g] = fmaf(8.0f, s.y, m.y);
+            }
+        }
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g)
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n)
+#pragma unroll
+                for (unsigned i = 0; i < 2; ++i) {  // hi + lo
+                    const float2 v = f2_unpack(o[g][n][i]);
+                    o[g][n][i] = add2(o[g][n][i], f2_pack(__shfl_xor_sync(0xffffffffu, v.x, 2),
+                                                          __shfl_xor_sync(0xffffffffu, v.y, 2)));
+                }
+    }
+    template <unsigned PITCH>
+    __device__ __forceinline__ void put_o(float* warp_o, unsigned rows) {
+        if (c < 2) put_columns<PITCH, D>(o, warp_o, 2 * c, rows, r);
+    }
+};
+
+// The tile's queries as operands of QK, each row scaled by a power of two to
+// about 2^9 at most and split into two fp16 parts. Warp w takes row w.
+template <typename T, unsigned D, typename Rows>
 __device__ __forceinline__ void load_queries(const AttnKv4Args& a, const Tile& t, unsigned head, Smem<D>& sm) {
     constexpr unsigned G = Shape<D>::groups;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const unsigned f = t.flat + warp;
+    if (warp >= Rows::ROWS) return;
     const bool have = warp < t.rows;
-    const T* q = static_cast<const T*>(a.q) + row_of(a, t, have ? f : t.flat) * a.q_row +
-                 (head * a.group + (have ? f : t.flat) % a.group) * a.q_head;
+    const unsigned f = t.flat + (have ? warp : 0u);
+    const T* q = static_cast<const T*>(a.q) + row_of(a, t, f) * a.q_row + (head * a.group + f % a.group) * a.q_head;
     float v[D / 32], top = 0.0f, sum[G];
 #pragma unroll
     for (unsigned g = 0; g < G; ++g) sum[g] = 0.0f;
 #pragma unroll
     for (unsigned e = 0; e < D / 32; ++e) {
-        v[e] = have ? as_float(q[lane + 32 * e]) : 0.0f;
+        v[e] = have ? as_float(q[lane + 32 * e]) * a.q_sign : 0.0f;
         top = fmaxf(top, fabsf(v[e]));
         sum[e / 2] += v[e];
     }
@@ -487,26 +905,22 @@ __device__ __forceinline__ void load_queries(const AttnKv4Args& a, const Tile& t
     for (unsigned g = 0; g < G; ++g) sum[g] = warp_sum(sum[g]);
     // 2^e with top * 2^e in [2^9, 2^10)
     int e = 136 - static_cast<int>(__float_as_uint(top) >> 23);
-    e = top == 0.0f || e < -100 ? (top == 0.0f ? 0 : -100) : min(e, 100);
+    e = top == 0.0f ? 0 : max(-100, min(e, 100));
     const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
     if (lane == 0) {
-        sm.q_scale[warp] = a.scale_log2 * __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+        // positive, so that a masked score stays -inf
+        sm.q_scale[warp] = fmaxf(a.scale_log2 * __uint_as_float(static_cast<unsigned>(127 - e) << 23), 1.17549435e-38f);
 #pragma unroll
-        for (unsigned g = 0; g < G; ++g) sm.q_sum[warp][g] = sum[g] * a.scale_log2;
+        for (unsigned g = 0; g < G; ++g) sm.q_sum[warp][g] = sum[g] * up;
     }
-    // dimension d = w * 32 + c * 8 + i of lane (row, c): nibble i of word w.
-    // Pair (i, i + 4) of one register.
-    __half* words = reinterpret_cast<__half*>(sm.q);
+    // dimension d = w * 32 + c * 8 + i: nibble i of word w of lane (row, c)
 #pragma unroll
     for (unsigned k = 0; k < D / 32; ++k) {
-        const unsigned d = lane + 32 * k, w = d / 32, c = d % 32 / 8, i = d % 8;
+        const unsigned c = lane / 8, i = lane % 8;
         const float x = v[k] * up;
         const __half hi = __float2half_rn(x);
         const __half lo = __float2half_rn(x - __half2float(hi));
-        const unsigned step = w * 2 + (i % 4) / 2, reg = (i & 1u) * 2, half = i / 4;
-        const unsigned at = ((step * 32 + warp * 4 + c) * 4 + reg) * 2 + half;
-        words[at] = hi;
-        words[at + 2] = lo;
+        Rows::put_query(sm, warp, k * 2 + (i % 4) / 2, c, i % 2, i / 4, hi, lo);
     }
 }
 
@@ -567,13 +981,12 @@ __device__ __forceinline__ void join_parts(const AttnKv4Args& a, const Tile& t, 
 
 // Units [from, to) of the pair (tile t of sequence seq, head): this CTA's
 // part. whole: they are all of it.
-template <typename T, unsigned D>
+template <typename T, unsigned D, typename Rows>
 __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t, unsigned seq, unsigned head,
                                             unsigned from, unsigned to, bool whole, std::size_t slot, Smem<D>& sm) {
     using S = Shape<D>;
-    constexpr unsigned G = S::groups;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    load_queries<T, D>(a, t, head, sm);
+    load_queries<T, D, Rows>(a, t, head, sm);
 
     const unsigned steps = to - from > warp ? (to - from - warp + kWarps - 1) / kWarps : 0u;
     const auto key_of = [&](unsigned i) { return (from + warp + i * kWarps) * kStep; };
@@ -590,36 +1003,16 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
     unsigned next_page = S::stages < steps ? lane_page(a, t, seq, key_of(S::stages) + lane) : kKv4Padding;
     __syncthreads();  // queries
 
-    const unsigned r = lane / 4;
-    const float q_scale = sm.q_scale[r];
-    float q_sum[G];
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) q_sum[g] = sm.q_sum[r][g];
-    const int pos = r < t.rows ? static_cast<int>(t.len) - static_cast<int>(t.queries) +
-                                     static_cast<int>((t.flat + r) / a.group)
-                               : -1;
-    WarpState<D> st;
-    st.ref = kNegInf;
-    st.sum = 0;
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-        st.mean[g] = 0;
-#pragma unroll
-        for (unsigned n = 0; n < 4; ++n) st.o[g][n][0] = st.o[g][n][1] = 0;
-    }
+    Rows rows;
+    rows.init(a, t, sm, lane);
     for (unsigned i = 0; i < steps; ++i) {
         cp_async_wait<S::stages - 1>();
         __syncwarp();
         const unsigned u0 = key_of(i), at = i % S::stages, stage = ring + at * S::stage;
         const unsigned valid = sm.valid[warp][at];
-        // all rows see all 32 keys: they exist, none is ahead of the first
-        // row, and none is behind the last row's window
-        const bool clear = valid == 0xFFFFFFFFu && static_cast<int>(key_position(t, u0 + kStep - 1)) <= t.p_min &&
-                           (a.window == 0 || u0 + kStep <= t.sinks ||
-                            static_cast<int>(u0 < t.sinks ? t.low : key_position(t, u0)) >
-                                t.p_max - static_cast<int>(a.window));
-        if (clear) attend_step<D, false>(a, t, sm, stage, u0, valid, pos, q_scale, q_sum, lane, st);
-        else attend_step<D, true>(a, t, sm, stage, u0, valid, pos, q_scale, q_sum, lane, st);
+        const bool clear = valid == 0xFFFFFFFFu && u0 >= t.clear_from && u0 + kStep <= t.clear_to;
+        if (clear) rows.template step<false>(a, t, sm, stage, u0, valid);
+        else rows.template step<true>(a, t, sm, stage, u0, valid);
         __syncwarp();
         if (i + S::stages < steps) {
             stage_step<D>(a, t, head, key_of(i + S::stages), next_page, stage, &sm.valid[warp][at], lane);
@@ -631,47 +1024,13 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
     cp_async_wait<0>();
 
     // ---- the warps' sums meet ----
-    const auto row_total = [](f32x2 v) {
-        const float2 y = f2_unpack(v);
-        float total = y.x + y.y;
-        total += __shfl_xor_sync(0xffffffffu, total, 1);
-        return total + __shfl_xor_sync(0xffffffffu, total, 2);
-    };
-    const float sum = row_total(st.sum);
-    float mean[G];
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) mean[g] = row_total(st.mean[g]);
-    if (lane % 4 == 0) {
-        sm.ref[warp][r] = st.ref;
-        sm.sum[warp][r] = sum;
-#pragma unroll
-        for (unsigned g = 0; g < G; ++g) sm.mean[warp][r][g] = mean[g];
-    }
+    rows.put_sums(sm, warp);
     __syncthreads();  // every ring is drained: it becomes the warps' O
     float* o = reinterpret_cast<float*>(sm.ring);
     constexpr unsigned PITCH = D + 4;
     const unsigned used = min(to - from, kWarps);  // warps that had a step
-    if (warp < used) {
-        const unsigned c2 = lane % 4 * 2;
-#pragma unroll
-        for (unsigned e = 0; e < 2; ++e)
-            if (c2 + e < t.rows) {
-                float* row = o + (warp * kRows + c2 + e) * PITCH + r * 8;
-#pragma unroll
-                for (unsigned g = 0; g < G; ++g) {
-                    float v[8];
-#pragma unroll
-                    for (unsigned n = 0; n < 4; ++n) {
-                        const float2 y0 = f2_unpack(st.o[g][n][0]), y1 = f2_unpack(st.o[g][n][1]);
-                        v[n] = e ? y0.y : y0.x;
-                        v[4 + n] = e ? y1.y : y1.x;
-                    }
-                    *reinterpret_cast<float4*>(row + g * 64) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4*>(row + g * 64 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                }
-            }
-    }
-    if (threadIdx.x < kRows) {
+    if (warp < used) rows.template put_o<PITCH>(o + warp * kRows * PITCH, t.rows);
+    if (threadIdx.x < Rows::ROWS) {
         float m = kNegInf, l = 0.0f;
         for (unsigned w = 0; w < used; ++w) m = fmaxf(m, sm.ref[w][threadIdx.x]);
         for (unsigned w = 0; w < used; ++w) {
@@ -729,12 +1088,12 @@ __device__ __forceinline__ bool scan_units(unsigned v, bool flag, Smem<D>& sm, u
 }
 
 // Zeros for this CTA's pairs of p0 .. p0 + kPairCache that see nothing.
-template <typename T, unsigned D>
+template <typename T, unsigned D, unsigned ROWS>
 __device__ __forceinline__ void write_blank_rows(const AttnKv4Args& a, unsigned p0) {
     const unsigned heads = a.cache.kv_heads, pairs = a.cache.seqs * a.tiles;
     const unsigned end = min(pairs, p0 + kPairCache);
     for (unsigned p = p0 + (blockIdx.x + gridDim.x - p0 % gridDim.x) % gridDim.x; p < end; p += gridDim.x) {
-        const Tile t = make_tile(a, p / a.tiles, p % a.tiles, false);
+        const Tile t = make_tile<ROWS>(a, p / a.tiles, p % a.tiles, false);
         if (t.total != 0) continue;
         for (unsigned i = threadIdx.x; i < t.rows * heads * D; i += kWarps * 32) {
             const unsigned f = t.flat + i / D / heads, h = i / D % heads;
@@ -744,7 +1103,7 @@ __device__ __forceinline__ void write_blank_rows(const AttnKv4Args& a, unsigned 
     }
 }
 
-template <typename T, unsigned D>
+template <typename T, unsigned D, typename Rows>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 attention_kv4_shares(AttnKv4Args a) {
     extern __shared__ unsigned char smem_raw[];
@@ -762,12 +1121,12 @@ attention_kv4_shares(AttnKv4Args a) {
         bool blank = false;  // rows that see nothing, this CTA's to write
         if (p < pairs) {
             const bool mine = p % gridDim.x == blockIdx.x;
-            const Tile t = make_tile(a, p / a.tiles, p % a.tiles, mine);
+            const Tile t = make_tile<Rows::ROWS>(a, p / a.tiles, p % a.tiles, mine);
             units = (t.total + kStep - 1) / kStep;
             blank = mine && units == 0 && t.rows;
         }
         unsigned before, total;
-        if (scan_units(units, blank, sm, &before, &total)) write_blank_rows<T, D>(a, p0);
+        if (scan_units(units, blank, sm, &before, &total)) write_blank_rows<T, D, Rows::ROWS>(a, p0);
         all_units += total;
         kept = units;
     }
@@ -791,7 +1150,7 @@ attention_kv4_shares(AttnKv4Args a) {
         unsigned units = kept;
         if (pairs > kPairCache) {
             units = 0;
-            if (p < pairs) units = (make_tile(a, p / a.tiles, p % a.tiles, false).total + kStep - 1) / kStep;
+            if (p < pairs) units = (make_tile<Rows::ROWS>(a, p / a.tiles, p % a.tiles, false).total + kStep - 1) / kStep;
         }
         unsigned before, total;
         scan_units(units, false, sm, &before, &total);
@@ -815,11 +1174,11 @@ attention_kv4_shares(AttnKv4Args a) {
         for (;; ++pair) {  // skips pairs that see nothing
             units = pair - block0 < kPairCache
                         ? sm.pair_units[pair - block0]
-                        : (make_tile(a, pair / a.tiles, pair % a.tiles, false).total + kStep - 1) / kStep;
+                        : (make_tile<Rows::ROWS>(a, pair / a.tiles, pair % a.tiles, false).total + kStep - 1) / kStep;
             if (units) break;
         }
         const unsigned seq = pair / a.tiles;
-        const Tile t = make_tile(a, seq, pair % a.tiles, false);
+        const Tile t = make_tile<Rows::ROWS>(a, seq, pair % a.tiles, false);
         while (at < stop && at < (pair_begin + units) * heads) {
             const unsigned head = static_cast<unsigned>((at - pair_begin * heads) / units);
             const unsigned long long begin = pair_begin * heads + static_cast<unsigned long long>(head) * units;
@@ -829,7 +1188,7 @@ attention_kv4_shares(AttnKv4Args a) {
             const bool whole = from == 0 && to == units;
             // a part at the start of the share goes to slot 0, one at its end to slot 1
             const std::size_t slot = static_cast<std::size_t>(2) * blockIdx.x + (from == 0 ? 1 : 0);
-            run_segment<T, D>(a, t, seq, head, from, to, whole, slot, sm);
+            run_segment<T, D, Rows>(a, t, seq, head, from, to, whole, slot, sm);
             if (!whole) {
                 const unsigned first = static_cast<unsigned>(begin / share);
                 const unsigned last = static_cast<unsigned>((end - 1) / share);
@@ -854,9 +1213,9 @@ attention_kv4_shares(AttnKv4Args a) {
     }
 }
 
-template <typename T, unsigned D>
+template <typename T, unsigned D, typename Rows>
 cudaError_t launch_attention(const AttnKv4Args& a, cudaStream_t s) {
-    auto kernel = attention_kv4_shares<T, D>;
+    auto kernel = attention_kv4_shares<T, D, Rows>;
     const std::size_t smem = sizeof(Smem<D>);
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
@@ -911,10 +1270,14 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride, v
     a.group = static_cast<unsigned>(q_heads / cache->kv_heads);
     a.q_offsets = q_offsets; a.lens = lens;
     a.max_queries = static_cast<unsigned>(max_queries); a.max_len = static_cast<unsigned>(max_len);
-    a.scale_log2 = scale * 1.4426950408889634f;
-    if (cache->seqs > 0x7FFFFFFFu / ((max_queries * a.group + kRows - 1) / kRows))
-        return invalid("b2_attention_kv4: too many row tiles");
-    a.tiles = static_cast<unsigned>((max_queries * a.group + kRows - 1) / kRows);
+    if (!(std::fabs(scale) < INFINITY)) return invalid("b2_attention_kv4: scale must be finite");
+    a.scale_log2 = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.4426950408889634f;
+    a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
+    // up to four rows of a KV head per sequence: the four-row form
+    const bool narrow = max_queries * a.group <= 4;
+    const std::size_t tiles = (max_queries * a.group + (narrow ? 3 : 7)) / (narrow ? 4 : 8);
+    if (cache->seqs > 0x7FFFFFFFu / tiles) return invalid("b2_attention_kv4: too many row tiles");
+    a.tiles = static_cast<unsigned>(tiles);
     a.counters = static_cast<unsigned*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.counters + kMaxGrid);
     a.part_o = a.part_ml + 2 * kMaxGrid * kRows * 2;
@@ -922,12 +1285,13 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride, v
     a.sinks = static_cast<unsigned>(sinks < 0x7FFFFFFFu ? sinks : 0x7FFFFFFFu);
     cudaStream_t s = as_stream(stream);
     cudaError_t e;
-    if (dtype == B2_DTYPE_F32) {
-        e = cache->head_dim == 128 ? launch_attention<float, 128>(a, s) : launch_attention<float, 64>(a, s);
-    } else {
-        e = cache->head_dim == 128 ? launch_attention<__nv_bfloat16, 128>(a, s)
-                                   : launch_attention<__nv_bfloat16, 64>(a, s);
-    }
+    const auto run = [&](auto element) {
+        using T = decltype(element);
+        if (cache->head_dim == 128)
+            return narrow ? launch_attention<T, 128, Narrow<128>>(a, s) : launch_attention<T, 128, Wide<128>>(a, s);
+        return narrow ? launch_attention<T, 64, Narrow<64>>(a, s) : launch_attention<T, 64, Wide<64>>(a, s);
+    };
+    e = dtype == B2_DTYPE_F32 ? run(float()) : run(__nv_bfloat16());
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(B2_ERR_CUDA, std::string("b2_attention_kv4: ") + cudaGetErrorString(e));
