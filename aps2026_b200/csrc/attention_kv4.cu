@@ -81,20 +81,19 @@ struct Shape {
     static constexpr unsigned codes = kStep * D / 2;          // bytes of a step's K (V) codes
     static constexpr unsigned params = kStep * 4 * groups;
     static constexpr unsigned stage = 2 * (codes + params);
-    static constexpr unsigned ring = kWarps * stages * stage;
 };
 
 template <unsigned D>
 struct Smem {
-    alignas(128) unsigned char ring[Shape<D>::ring];  // also the warps' O at a segment's end
+    alignas(128) unsigned char ring[kWarps][Shape<D>::stages * Shape<D>::stage];  // also a warp's O at a segment's end
     alignas(16) __half q[D / 16][32][8];              // operands of QK: k-step, lane (4 halves used by Narrow)
     float q_sum[kRows][2];                            // sum of the scaled q per group
     float q_scale[kRows];                             // base-2 score per unit of product with the scaled q
     unsigned valid[kWarps][Shape<D>::stages];         // positions of the step that exist
     float ref[kWarps][kRows], sum[kWarps][kRows], mean[kWarps][kRows][2];
-    float row_ref[kRows], row_sum[kRows];
+    float row_sum[kRows];
     unsigned pair_units[kPairCache];
-    unsigned scan[kWarps], scan_total, found_pair, found_before, last;
+    unsigned scan[kWarps], fits[kWarps], found_pair, found_before, last;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, unsigned b0, unsigned b1) {
@@ -420,10 +419,9 @@ struct Wide {
         at[2] = lo;
     }
 
-    // MASKED: some row does not see some of the keys.
-    template <bool MASKED>
+    // clear: every row sees all of the keys.
     __device__ __forceinline__ void step(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned stage,
-                                         unsigned u0, unsigned valid) {
+                                         unsigned u0, unsigned valid, bool clear) {
         // ---- scores: x[b] holds keys 8b + 2c and 8b + 2c + 1 of row r ----
         f32x2 x[4];
         {
@@ -464,7 +462,7 @@ struct Wide {
         unsigned vp[4][2 * G];
 #pragma unroll
         for (unsigned b = 0; b < 4; ++b) lds_n<2 * G>(stage + 2 * S::codes + S::params + (8 * b + 2 * c) * 4 * G, vp[b]);
-        if (MASKED) {
+        if (!clear) {
 #pragma unroll
             for (unsigned b = 0; b < 4; ++b) {
                 float2 y = f2_unpack(x[b]);
@@ -665,9 +663,8 @@ struct Narrow {
         sm.q[step][(row + ROWS) * 4 + c][reg * 2 + half] = lo;
     }
 
-    template <bool MASKED>
     __device__ __forceinline__ void step(const AttnKv4Args& a, const Tile& t, const Smem<D>&, unsigned stage, unsigned u0,
-                                         unsigned valid) {
+                                         unsigned valid, bool clear) {
         const bool upper = c & 2u;
         // ---- scores: y[k][h] is key 16k + 8h + r, columns 2c and 2c + 1 ----
         f32x2 y[2][2];
@@ -712,7 +709,7 @@ struct Narrow {
                                                            __shfl_xor_sync(0xffffffffu, give.y, 2)));
             lds_n<G>(stage + 2 * S::codes + S::params + (first + 8 * h) * 4 * G, vp[h]);
         }
-        if (MASKED) {
+        if (!clear) {
 #pragma unroll
             for (unsigned h = 0; h < 2; ++h) {
                 const unsigned tok = first + 8 * h;
@@ -882,21 +879,29 @@ struct Narrow {
 };
 
 // The tile's queries as operands of QK, each row scaled by a power of two to
-// about 2^9 at most and split into two fp16 parts. Warp w takes row w.
-template <typename T, unsigned D, typename Rows>
-__device__ __forceinline__ void load_queries(const AttnKv4Args& a, const Tile& t, unsigned head, Smem<D>& sm) {
+// about 2^9 at most and split into two fp16 parts. Warp w takes row w: lane's
+// dimensions are lane, lane + 32, ...
+template <typename T, unsigned D, unsigned ROWS>
+__device__ __forceinline__ void fetch_query(const AttnKv4Args& a, const Tile& t, unsigned head, float (&v)[D / 32]) {
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+#pragma unroll
+    for (unsigned e = 0; e < D / 32; ++e) v[e] = 0.0f;
+    if (warp >= t.rows) return;
+    const unsigned f = t.flat + warp;
+    const T* q = static_cast<const T*>(a.q) + row_of(a, t, f) * a.q_row + (head * a.group + f % a.group) * a.q_head;
+#pragma unroll
+    for (unsigned e = 0; e < D / 32; ++e) v[e] = as_float(q[lane + 32 * e]) * a.q_sign;
+}
+template <unsigned D, typename Rows>
+__device__ __forceinline__ void place_query(const AttnKv4Args& a, const float (&v)[D / 32], Smem<D>& sm) {
     constexpr unsigned G = Shape<D>::groups;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     if (warp >= Rows::ROWS) return;
-    const bool have = warp < t.rows;
-    const unsigned f = t.flat + (have ? warp : 0u);
-    const T* q = static_cast<const T*>(a.q) + row_of(a, t, f) * a.q_row + (head * a.group + f % a.group) * a.q_head;
-    float v[D / 32], top = 0.0f, sum[G];
+    float top = 0.0f, sum[G];
 #pragma unroll
     for (unsigned g = 0; g < G; ++g) sum[g] = 0.0f;
 #pragma unroll
     for (unsigned e = 0; e < D / 32; ++e) {
-        v[e] = have ? as_float(q[lane + 32 * e]) * a.q_sign : 0.0f;
         top = fmaxf(top, fabsf(v[e]));
         sum[e / 2] += v[e];
     }
@@ -930,53 +935,98 @@ __device__ __forceinline__ void store_out(T* p, float y) {
     else *p = y;
 }
 
-// Adds up the parts of a pair that CTAs first .. last hold (in this order)
-// and writes its rows. `begin`: first unit of the pair in the list.
+// Adds up the parts of a pair that CTAs first .. first + n - 1 hold, in this
+// order, and writes its rows.
 template <typename T, unsigned D>
-__device__ __forceinline__ void join_parts(const AttnKv4Args& a, const Tile& t, unsigned head, unsigned long long begin,
-                                           unsigned long long share, unsigned first, unsigned last, Smem<D>& sm) {
-    const unsigned n = last - first + 1;
-    float* factor = reinterpret_cast<float*>(sm.ring);  // [8][n]
+__device__ __forceinline__ void join_parts(const AttnKv4Args& a, const Tile& t, unsigned head, unsigned first, unsigned n,
+                                           Smem<D>& sm) {
+    constexpr unsigned FEW = 4;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const auto slot = [&](unsigned i) {
-        return static_cast<std::size_t>(2) * (first + i) + (begin < (first + i) * share ? 0 : 1);
+    const auto slot = [&](unsigned i) { return static_cast<std::size_t>(2) * (first + i) + (i == 0 ? 1u : 0u); };
+    const float4* parts = reinterpret_cast<const float4*>(a.part_o);
+    const float2* refs = reinterpret_cast<const float2*>(a.part_ml);
+    const auto write = [&](unsigned row, unsigned d4, const float4& s, float l) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const unsigned f = t.flat + row;
+        T* out = static_cast<T*>(a.out) + (row_of(a, t, f) * a.q_heads + head * a.group + f % a.group) * D + d4 * 4;
+        // a row without keys has s = 0 and l = 0
+        store_out(out, s.x * inv);
+        store_out(out + 1, s.y * inv);
+        store_out(out + 2, s.z * inv);
+        store_out(out + 3, s.w * inv);
     };
+    const auto add = [](float4& s, float w, const float4& v) {
+        s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+    };
+    if (n <= FEW) {  // everything in flight at once
+        for (unsigned i = threadIdx.x; i < t.rows * (D / 4); i += kWarps * 32) {
+            const unsigned row = i / (D / 4), d4 = i % (D / 4);
+            float2 ml[FEW];
+            float4 v[FEW];
+#pragma unroll
+            for (unsigned k = 0; k < FEW; ++k)
+                if (k < n) {
+                    ml[k] = __ldcg(refs + slot(k) * kRows + row);
+                    v[k] = __ldcg(parts + (slot(k) * kRows + row) * (D / 4) + d4);
+                } else {
+                    ml[k] = make_float2(kNegInf, 0.0f);
+                    v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            float m = kNegInf, l = 0.0f;
+#pragma unroll
+            for (unsigned k = 0; k < FEW; ++k) m = fmaxf(m, ml[k].x);
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (unsigned k = 0; k < FEW; ++k) {
+                const float w = ml[k].x == kNegInf ? 0.0f : exp2_approx(ml[k].x - m);
+                l = fmaf(w, ml[k].y, l);
+                if (w != 0.0f) add(s, w, v[k]);
+            }
+            write(row, d4, s, l);
+        }
+        return;
+    }
+    float* factor = reinterpret_cast<float*>(sm.ring);  // [rows][n]
     if (warp < t.rows) {
         float m = kNegInf, l = 0.0f;
         for (unsigned i = lane; i < n; i += 32) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot(i) * kRows + warp);
-            factor[warp * n + i] = v.x;
-            m = fmaxf(m, v.x);
+            const float x = __ldcg(&refs[slot(i) * kRows + warp].x);
+            factor[warp * n + i] = x;
+            m = fmaxf(m, x);
         }
         m = warp_max(m);
         for (unsigned i = lane; i < n; i += 32) {
             const float ref = factor[warp * n + i];
             const float w = ref == kNegInf ? 0.0f : exp2_approx(ref - m);
             factor[warp * n + i] = w;
-            l += w * __ldcg(a.part_ml + (slot(i) * kRows + warp) * 2 + 1);
+            l += w * __ldcg(&refs[slot(i) * kRows + warp].y);
         }
         l = warp_sum(l);
         if (lane == 0) sm.row_sum[warp] = l;
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < t.rows * (D / 4); i += kWarps * 32) {
-        const unsigned row = i / (D / 4), d4 = i % (D / 4);
+    // the parts are cut among the threads that a row's outputs leave idle, and added in order
+    const unsigned outputs = t.rows * (D / 4);
+    const unsigned cuts = max(1u, min(kWarps * 32 / outputs, 8u)), per = (n + cuts - 1) / cuts;
+    float4* sums = reinterpret_cast<float4*>(sm.ring) + (kRows * kMaxGrid) / 4;  // [cuts][outputs]
+    for (unsigned i = threadIdx.x; i < outputs * cuts; i += kWarps * 32) {
+        const unsigned cut = i / outputs, o = i % outputs, row = o / (D / 4), d4 = o % (D / 4);
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (unsigned k = 0; k < n; ++k) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o) + (slot(k) * kRows + row) * (D / 4) + d4);
+        const unsigned end = min(n, (cut + 1) * per);
+#pragma unroll 10
+        for (unsigned k = cut * per; k < end; ++k) {
+            const float4 v = __ldcg(parts + (slot(k) * kRows + row) * (D / 4) + d4);
             const float w = factor[row * n + k];
-            s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+            if (w != 0.0f) add(s, w, v);
         }
-        const float l = sm.row_sum[row], inv = 1.0f / l;
-        const unsigned f = t.flat + row;
-        T* out = static_cast<T*>(a.out) + (row_of(a, t, f) * a.q_heads + head * a.group + f % a.group) * D + d4 * 4;
-        store_out(out, l == 0.0f ? 0.0f : s.x * inv);
-        store_out(out + 1, l == 0.0f ? 0.0f : s.y * inv);
-        store_out(out + 2, l == 0.0f ? 0.0f : s.z * inv);
-        store_out(out + 3, l == 0.0f ? 0.0f : s.w * inv);
+        sums[cut * outputs + o] = s;
     }
     __syncthreads();
+    for (unsigned o = threadIdx.x; o < outputs; o += kWarps * 32) {
+        float4 s = sums[o];
+        for (unsigned cut = 1; cut < cuts; ++cut) add(s, 1.0f, sums[cut * outputs + o]);
+        write(o / (D / 4), o % (D / 4), s, sm.row_sum[o / (D / 4)]);
+    }
 }
 
 // Units [from, to) of the pair (tile t of sequence seq, head): this CTA's
@@ -986,21 +1036,24 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
                                             unsigned from, unsigned to, bool whole, std::size_t slot, Smem<D>& sm) {
     using S = Shape<D>;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    load_queries<T, D, Rows>(a, t, head, sm);
 
     const unsigned steps = to - from > warp ? (to - from - warp + kWarps - 1) / kWarps : 0u;
     const auto key_of = [&](unsigned i) { return (from + warp + i * kWarps) * kStep; };
-    const unsigned ring = smem_addr(sm.ring) + warp * S::stages * S::stage;
-    unsigned pages[S::stages];
+    const unsigned ring = smem_addr(sm.ring[warp]);
+    // page numbers, then queries, then keys: each latency starts as early as it can
+    unsigned pages[S::stages], next_page = kKv4Padding;
 #pragma unroll
     for (unsigned i = 0; i < S::stages; ++i)
         pages[i] = i < steps ? lane_page(a, t, seq, key_of(i) + lane) : kKv4Padding;
+    float query[D / 32];
+    fetch_query<T, D, Rows::ROWS>(a, t, head, query);
 #pragma unroll
     for (unsigned i = 0; i < S::stages; ++i) {
         if (i < steps) stage_step<D>(a, t, head, key_of(i), pages[i], ring + i * S::stage, &sm.valid[warp][i], lane);
         cp_async_commit();
     }
-    unsigned next_page = S::stages < steps ? lane_page(a, t, seq, key_of(S::stages) + lane) : kKv4Padding;
+    if (S::stages < steps) next_page = lane_page(a, t, seq, key_of(S::stages) + lane);
+    place_query<D, Rows>(a, query, sm);
     __syncthreads();  // queries
 
     Rows rows;
@@ -1011,8 +1064,7 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
         const unsigned u0 = key_of(i), at = i % S::stages, stage = ring + at * S::stage;
         const unsigned valid = sm.valid[warp][at];
         const bool clear = valid == 0xFFFFFFFFu && u0 >= t.clear_from && u0 + kStep <= t.clear_to;
-        if (clear) rows.template step<false>(a, t, sm, stage, u0, valid);
-        else rows.template step<true>(a, t, sm, stage, u0, valid);
+        rows.step(a, t, sm, stage, u0, valid, clear);
         __syncwarp();
         if (i + S::stages < steps) {
             stage_step<D>(a, t, head, key_of(i + S::stages), next_page, stage, &sm.valid[warp][at], lane);
@@ -1024,42 +1076,47 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
     cp_async_wait<0>();
 
     // ---- the warps' sums meet ----
-    rows.put_sums(sm, warp);
-    __syncthreads();  // every ring is drained: it becomes the warps' O
-    float* o = reinterpret_cast<float*>(sm.ring);
-    constexpr unsigned PITCH = D + 4;
     const unsigned used = min(to - from, kWarps);  // warps that had a step
-    if (warp < used) rows.template put_o<PITCH>(o + warp * kRows * PITCH, t.rows);
-    if (threadIdx.x < Rows::ROWS) {
-        float m = kNegInf, l = 0.0f;
-        for (unsigned w = 0; w < used; ++w) m = fmaxf(m, sm.ref[w][threadIdx.x]);
-        for (unsigned w = 0; w < used; ++w) {
-            const float ref = sm.ref[w][threadIdx.x];
-            const float f = ref == kNegInf ? 0.0f : exp2_approx(ref - m);
-            sm.ref[w][threadIdx.x] = f;
-            l += f * sm.sum[w][threadIdx.x];
-        }
-        sm.row_ref[threadIdx.x] = m;
-        sm.row_sum[threadIdx.x] = l;
+    constexpr unsigned PITCH = D + 4;
+    float* o = reinterpret_cast<float*>(sm.ring[0]);
+    static_assert(kRows * PITCH * sizeof(float) <= sizeof(sm.ring[0]), "a warp's O fits its own ring");
+    if (warp < used) {
+        rows.put_sums(sm, warp);
+        __syncwarp();
+        // the warp's ring is drained: it becomes its O
+        rows.template put_o<PITCH>(reinterpret_cast<float*>(sm.ring[warp]), t.rows);
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < t.rows * D; i += kWarps * 32) {
-        const unsigned row = i / D, d = i % D;
-        float y = 0.0f;
-        for (unsigned w = 0; w < used; ++w)
-            y = fmaf(sm.ref[w][row], o[(w * kRows + row) * PITCH + d] + sm.mean[w][row][d / kKv4Group], y);
+    constexpr unsigned APART = sizeof(sm.ring[0]) / sizeof(float);
+    for (unsigned i = threadIdx.x; i < t.rows * (D / 4); i += kWarps * 32) {
+        const unsigned row = i / (D / 4), d = i % (D / 4) * 4;
+        float m = kNegInf, l = 0.0f;
+        for (unsigned w = 0; w < used; ++w) m = fmaxf(m, sm.ref[w][row]);
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (unsigned w = 0; w < used; ++w) {
+            const float ref = sm.ref[w][row];
+            const float f = ref == kNegInf ? 0.0f : exp2_approx(ref - m);
+            const float4 v = *reinterpret_cast<const float4*>(o + w * APART + row * PITCH + d);
+            const float mean = sm.mean[w][row][d / kKv4Group];
+            l = fmaf(f, sm.sum[w][row], l);
+            y.x = fmaf(f, v.x + mean, y.x);
+            y.y = fmaf(f, v.y + mean, y.y);
+            y.z = fmaf(f, v.z + mean, y.z);
+            y.w = fmaf(f, v.w + mean, y.w);
+        }
         if (whole) {
             const unsigned f = t.flat + row;
-            const float l = sm.row_sum[row];
-            store_out(static_cast<T*>(a.out) + (row_of(a, t, f) * a.q_heads + head * a.group + f % a.group) * D + d,
-                      l == 0.0f ? 0.0f : y / l);
+            T* out = static_cast<T*>(a.out) + (row_of(a, t, f) * a.q_heads + head * a.group + f % a.group) * D + d;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no keys: y = 0 too
+            store_out(out, y.x * inv);
+            store_out(out + 1, y.y * inv);
+            store_out(out + 2, y.z * inv);
+            store_out(out + 3, y.w * inv);
         } else {
-            __stcg(a.part_o + (slot * kRows + row) * D + d, y);
+            __stcg(reinterpret_cast<float4*>(a.part_o + (slot * kRows + row) * D + d), y);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(a.part_ml) + slot * kRows + row, make_float2(m, l));
         }
     }
-    if (!whole && threadIdx.x < t.rows)
-        __stcg(reinterpret_cast<float2*>(a.part_ml) + slot * kRows + threadIdx.x,
-               make_float2(sm.row_ref[threadIdx.x], sm.row_sum[threadIdx.x]));
 }
 
 // Exclusive sum of v over the CTA's threads and the total, through sm.scan;
@@ -1103,6 +1160,53 @@ __device__ __forceinline__ void write_blank_rows(const AttnKv4Args& a, unsigned 
     }
 }
 
+// One part of a pair: units [from, to) of (pair, head), which CTAs first ..
+// first + n - 1 share.
+struct Part {
+    unsigned pair, head, from, to, first, n;
+};
+
+template <typename T, unsigned D, typename Rows>
+__device__ __forceinline__ void run_part(const AttnKv4Args& a, const Part& p, Smem<D>& sm) {
+    const unsigned seq = p.pair / a.tiles;
+    const Tile t = make_tile<Rows::ROWS>(a, seq, p.pair % a.tiles, false);
+    // the slot of a pair's first part is the CTA's second: it may also hold the end of another pair
+    const std::size_t slot = static_cast<std::size_t>(2) * blockIdx.x + (p.from == 0 ? 1 : 0);
+    run_segment<T, D, Rows>(a, t, seq, p.head, p.from, p.to, p.n == 1, slot, sm);
+    if (p.n > 1) {
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sm.last = atomicAdd(a.counters + p.first, 1u) == p.n - 1;
+            if (sm.last) a.counters[p.first] = 0;
+        }
+        __syncthreads();
+        if (sm.last) {
+            __threadfence();
+            join_parts<T, D>(a, t, p.head, p.first, p.n, sm);
+        }
+    }
+    __syncthreads();  // the next part overwrites what this one used
+}
+
+// Each pair on CTAs of its own, as few as keep every CTA at `most` units:
+// sum over pairs of ceil(units / most) * heads CTAs. Returns the least of
+// kWarps candidates for `most` that fits the grid (0: none does). One warp
+// tries one candidate.
+template <unsigned D>
+__device__ __forceinline__ unsigned fit_pairs(unsigned pairs, unsigned heads, unsigned share, Smem<D>& sm) {
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const unsigned most = share + warp * 2;
+    unsigned ctas = 0;
+    for (unsigned p = lane; p < pairs; p += 32) ctas += (sm.pair_units[p] + most - 1) / most;
+    ctas = __reduce_add_sync(0xffffffffu, ctas) * heads;
+    if (lane == 0) sm.fits[warp] = ctas <= gridDim.x;
+    __syncthreads();
+    for (unsigned w = 0; w < kWarps; ++w)
+        if (sm.fits[w]) return share + w * 2;
+    return 0;
+}
+
 template <typename T, unsigned D, typename Rows>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 attention_kv4_shares(AttnKv4Args a) {
@@ -1111,13 +1215,16 @@ attention_kv4_shares(AttnKv4Args a) {
     pdl_begin();
     const unsigned heads = a.cache.kv_heads;
     const unsigned pairs = a.cache.seqs * a.tiles;
+    const auto units_of = [&](unsigned pair) {
+        return (make_tile<Rows::ROWS>(a, pair / a.tiles, pair % a.tiles, false).total + kStep - 1) / kStep;
+    };
 
     // ---- sizes of all pairs; rows that see nothing are written here ----
     unsigned long long all_units = 0;
-    unsigned kept = 0;  // units of pair threadIdx.x, for pairs <= kPairCache
+    unsigned units = 0, before = 0, total = 0;  // of pair threadIdx.x, when there are up to kPairCache
     for (unsigned p0 = 0; p0 < pairs; p0 += kPairCache) {
         const unsigned p = p0 + threadIdx.x;
-        unsigned units = 0;
+        units = 0;
         bool blank = false;  // rows that see nothing, this CTA's to write
         if (p < pairs) {
             const bool mine = p % gridDim.x == blockIdx.x;
@@ -1125,13 +1232,10 @@ attention_kv4_shares(AttnKv4Args a) {
             units = (t.total + kStep - 1) / kStep;
             blank = mine && units == 0 && t.rows;
         }
-        unsigned before, total;
+        sm.pair_units[threadIdx.x] = units;
         if (scan_units(units, blank, sm, &before, &total)) write_blank_rows<T, D, Rows::ROWS>(a, p0);
         all_units += total;
-        kept = units;
     }
-
-    // ---- this CTA's share of the list (pair-major, then head, then unit) ----
     const unsigned long long work = all_units * heads;
     unsigned long long share = (work + gridDim.x - 1) / gridDim.x;
     // short contexts: not less than a pair, up to a unit per warp, so that a
@@ -1139,77 +1243,79 @@ attention_kv4_shares(AttnKv4Args a) {
     const unsigned long long per_pair = (work + static_cast<unsigned long long>(pairs) * heads - 1) /
                                         (static_cast<unsigned long long>(pairs) * heads);
     share = max(share, min(per_pair, static_cast<unsigned long long>(kWarps)));
-    unsigned long long at = blockIdx.x * share;
-    const unsigned long long stop = min(at + share, work);
-    if (at >= stop) return;
-    // the pair that holds unit `at`
-    unsigned long long pair_begin = 0;  // units of earlier pairs, one head
-    unsigned block0 = 0;                // first pair of the cached block
-    for (unsigned p0 = 0; p0 < pairs; p0 += kPairCache) {
-        const unsigned p = p0 + threadIdx.x;
-        unsigned units = kept;
-        if (pairs > kPairCache) {
-            units = 0;
-            if (p < pairs) units = (make_tile<Rows::ROWS>(a, p / a.tiles, p % a.tiles, false).total + kStep - 1) / kStep;
-        }
-        unsigned before, total;
-        scan_units(units, false, sm, &before, &total);
-        sm.pair_units[threadIdx.x] = units;
-        const unsigned long long b = (pair_begin + before) * heads;
-        if (units && at >= b && at < b + static_cast<unsigned long long>(units) * heads) {
-            sm.found_pair = p;
+
+    // ---- pairs on CTAs of their own, if that leaves no CTA with much more
+    // than its share: a second part costs a CTA what some 16 units do ----
+    Part part;
+    unsigned long long at = 0, stop = 0;  // else: the CTA's share of the list
+    unsigned long long pair_begin = 0;    // units of earlier pairs, one head
+    unsigned block0 = 0;                  // first pair of the cached block
+    unsigned most = 0;
+    if (pairs <= kPairCache && static_cast<unsigned long long>(pairs) * heads <= gridDim.x && share < 0x10000000u)
+        most = fit_pairs<D>(pairs, heads, static_cast<unsigned>(share), sm);
+    if (most) {
+        const unsigned n = (units + most - 1) / most;  // CTAs of this thread's pair, per head
+        scan_units(n, false, sm, &before, &total);
+        const unsigned b = blockIdx.x;
+        if (b >= total * heads) return;
+        if (n && b >= before * heads && b < (before + n) * heads) {
+            sm.found_pair = threadIdx.x;
             sm.found_before = before;
         }
         __syncthreads();
-        block0 = p0;
-        if (at < (pair_begin + total) * heads) {
-            pair_begin += sm.found_before;
-            break;
-        }
-        pair_begin += total;
-    }
-    unsigned pair = sm.found_pair;
-    while (at < stop) {
-        unsigned units = 0;
-        for (;; ++pair) {  // skips pairs that see nothing
-            units = pair - block0 < kPairCache
-                        ? sm.pair_units[pair - block0]
-                        : (make_tile<Rows::ROWS>(a, pair / a.tiles, pair % a.tiles, false).total + kStep - 1) / kStep;
-            if (units) break;
-        }
-        const unsigned seq = pair / a.tiles;
-        const Tile t = make_tile<Rows::ROWS>(a, seq, pair % a.tiles, false);
-        while (at < stop && at < (pair_begin + units) * heads) {
-            const unsigned head = static_cast<unsigned>((at - pair_begin * heads) / units);
-            const unsigned long long begin = pair_begin * heads + static_cast<unsigned long long>(head) * units;
-            const unsigned long long end = begin + units;
-            const unsigned from = static_cast<unsigned>(at - begin);
-            const unsigned to = static_cast<unsigned>(min(end, stop) - begin);
-            const bool whole = from == 0 && to == units;
-            // a part at the start of the share goes to slot 0, one at its end to slot 1
-            const std::size_t slot = static_cast<std::size_t>(2) * blockIdx.x + (from == 0 ? 1 : 0);
-            run_segment<T, D, Rows>(a, t, seq, head, from, to, whole, slot, sm);
-            if (!whole) {
-                const unsigned first = static_cast<unsigned>(begin / share);
-                const unsigned last = static_cast<unsigned>((end - 1) / share);
-                __threadfence();
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    const unsigned arrived = atomicAdd(a.counters + first, 1u);
-                    sm.last = arrived == last - first;
-                    if (sm.last) a.counters[first] = 0;
-                }
-                __syncthreads();
-                if (sm.last) {
-                    __threadfence();
-                    join_parts<T, D>(a, t, head, begin, share, first, last, sm);
-                }
+        part.pair = sm.found_pair;
+        const unsigned all = sm.pair_units[part.pair], cut = (all + most - 1) / most;
+        const unsigned k = b - sm.found_before * heads, index = k % cut, each = (all + cut - 1) / cut;
+        part.head = k / cut;
+        part.n = (all + each - 1) / each;
+        part.first = b - index;
+        part.from = index * each;
+        part.to = min(all, part.from + each);
+        if (index >= part.n) return;
+    } else {
+        at = blockIdx.x * share;
+        stop = min(at + share, work);
+        if (at >= stop) return;
+        for (unsigned p0 = 0; p0 < pairs; p0 += kPairCache) {
+            const unsigned p = p0 + threadIdx.x;
+            if (pairs > kPairCache) {
+                units = p < pairs ? units_of(p) : 0u;
+                scan_units(units, false, sm, &before, &total);
+                sm.pair_units[threadIdx.x] = units;
             }
-            __syncthreads();  // the next segment's queries overwrite these
-            at = begin + to;
+            const unsigned long long b = (pair_begin + before) * heads;
+            if (units && at >= b && at < b + static_cast<unsigned long long>(units) * heads) {
+                sm.found_pair = p;
+                sm.found_before = before;
+            }
+            __syncthreads();
+            block0 = p0;
+            if (at < (pair_begin + total) * heads) {
+                pair_begin += sm.found_before;
+                break;
+            }
+            pair_begin += total;
         }
-        pair_begin += units;
-        ++pair;
+        part.pair = sm.found_pair;
+    }
+    for (;;) {
+        if (!most) {  // the list's part at unit `at`
+            unsigned size = 0;
+            for (;; ++part.pair) {  // skips pairs that see nothing
+                size = part.pair - block0 < kPairCache ? sm.pair_units[part.pair - block0] : units_of(part.pair);
+                if (at < (pair_begin + size) * heads) break;
+                pair_begin += size;
+            }
+            part.head = static_cast<unsigned>((at - pair_begin * heads) / size);
+            const unsigned long long begin = pair_begin * heads + static_cast<unsigned long long>(part.head) * size;
+            part.from = static_cast<unsigned>(at - begin);
+            part.to = static_cast<unsigned>(min(begin + size, stop) - begin);
+            part.first = static_cast<unsigned>(begin / share);
+            part.n = static_cast<unsigned>((begin + size - 1) / share) - part.first + 1;
+            at = begin + part.to;
+        }
+        run_part<T, D, Rows>(a, part, sm);
+        if (most || at >= stop) break;
     }
 }
 
