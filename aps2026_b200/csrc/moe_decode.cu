@@ -16,15 +16,16 @@
 // fp32 weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
 // truncates, so chains are short (2 blocks) and added in registers.
 //
-// Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens,
-// 8 MT rows of gate and the same of up); a CTA takes equally many items, one
+// Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens, 8
+// rows of gate and the same of up); a CTA takes equally many items, one
 // after the other through the same rings. Its warps interleave the k blocks,
-// so together they read whole lines, and add up in shared memory. Launch 2,
-// moe_down: CTA = 16 rows of the output for all tokens; warps take (expert,
-// token chunk, part of k) and meet in shared memory, where a token's two
-// experts are summed in ascending order: no atomics, results repeat. Each
-// CTA routes for itself (T x E logits). Launch 2 starts under launch 1 and
-// has routed and requested its first weights before it waits.
+// so together they read whole lines, and add up in shared memory. It leaves
+// the activations in their parts. Launch 2, moe_down: CTA = 16 MT rows of the
+// output for all tokens; warps take (expert, 8 of its tokens, part of k) and
+// meet in shared memory, where a token's two experts are summed in ascending
+// order: no float atomics, results repeat. Each CTA routes for itself (T x E
+// logits). Launch 2 starts under launch 1 and has routed and requested its
+// first weights before it waits.
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -35,10 +36,11 @@ namespace b2 {
 namespace {
 
 constexpr unsigned kMaxDecodeTokens = 128;
-constexpr unsigned kMaxGroups = kMaxExperts + 2 * kMaxDecodeTokens / 16;
+constexpr unsigned kMaxGroups = kMaxExperts + 2 * kMaxDecodeTokens / 8;
 constexpr unsigned kChain = 2;           // blocks between two additions in registers
 constexpr unsigned kDownPartials = 256;  // (part of k, assignment) sums of moe_down
-constexpr unsigned kUpRing = 8192, kDownRing = 10240;  // bytes of a warp's stages
+constexpr unsigned kWarps = 16;          // one CTA per SM: all its shared memory is rings
+constexpr unsigned kRing = 11264;        // bytes of a warp's stages
 
 struct MoeDecodeArgs {
     const void* x;
@@ -51,69 +53,104 @@ struct MoeDecodeArgs {
     const void* w_down;
     void* out;
     std::size_t ld_out;
-    float* act;       // [2T, act_ld]: assignment 2t + s, s = 0 the lower expert
+    void* act;        // [parts][2T][act_ld]: assignment 2t + s, s = 0 the lower expert
     unsigned act_ld;  // I rounded up to 8; zeros past I
 };
 
 // ---- routing, per CTA ----------------------------------------------------------
 
 struct Plan {
-    unsigned mask[kMaxDecodeTokens / 32][kMaxExperts];     // tokens of each expert, by bit
-    unsigned char lists[kMaxExperts][kMaxDecodeTokens];    // assignments of each expert, tokens ascending
+    unsigned mask[kMaxDecodeTokens / 32][kMaxExperts];   // tokens of each expert, by bit
+    unsigned char lists[kMaxExperts][kMaxDecodeTokens];  // assignments of each expert, tokens ascending
+    unsigned short pair[kMaxDecodeTokens];               // lower expert | higher << 8
     float gate[2 * kMaxDecodeTokens];
-    unsigned group[kMaxGroups];                            // expert | first in list << 8 | count << 16
+    unsigned group[kMaxGroups];                          // expert | first in list << 8 | count << 16
     unsigned groups;
 };
 __device__ __forceinline__ unsigned group_expert(unsigned g) { return g & 0xFFu; }
 __device__ __forceinline__ unsigned group_first(unsigned g) { return (g >> 8) & 0xFFu; }
 __device__ __forceinline__ unsigned group_count(unsigned g) { return g >> 16; }
 
-// Routes the tokens and cuts every expert's into groups of CHUNK. THREADS >=
-// 256. Ends with a barrier.
+// The expert that b2_moe_route's ascending scan ends with, among those of
+// `alive` (one lane per expert, SUB lanes per token, score: this lane's): it
+// starts with the lowest and moves to the next one that beats it by more than
+// tie_eps. Each step of the loop is one such move.
+template <unsigned SUB>
+__device__ __forceinline__ unsigned scan_best(float score, unsigned lane, unsigned alive, float tie_eps) {
+    const unsigned base = lane / SUB * SUB;
+    const unsigned mine = SUB == 32 ? alive : (alive >> base) & 0xFFFFu;
+    unsigned best = __ffs(mine) - 1;  // two are alive at least
+    for (;;) {
+        const float bar = __fadd_rn(__shfl_sync(0xffffffffu, score, base + best), tie_eps);
+        const unsigned beats = __ballot_sync(0xffffffffu, score > bar) & alive;
+        const unsigned after = (SUB == 32 ? beats : (beats >> base) & 0xFFFFu) & (0xFFFFFFFEu << best);
+        if (after) best = __ffs(after) - 1;
+        if (!__any_sync(0xffffffffu, after != 0)) return best;
+    }
+}
+
+// A lane per expert, 32 / SUB tokens per warp at a time: the code stays short
+// (it runs once per CTA, from a cold instruction cache).
+template <unsigned SUB>
+__device__ __forceinline__ void pick_experts(const MoeDecodeArgs& a, Plan& p) {
+    constexpr unsigned AT_ONCE = 32 / SUB, BATCH = 4;
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, e = lane % SUB;
+    for (unsigned t0 = warp * AT_ONCE; t0 < a.T; t0 += kWarps * AT_ONCE * BATCH) {
+        float raw[BATCH];
+#pragma unroll
+        for (unsigned i = 0; i < BATCH; ++i) {
+            const unsigned t = t0 + i * kWarps * AT_ONCE + lane / SUB;
+            raw[i] = t < a.T && e < a.E ? __ldg(a.logits + static_cast<std::size_t>(t) * a.E + e) : 0.0f;
+        }
+#pragma unroll 1
+        for (unsigned i = 0; i < BATCH && t0 + i * kWarps * AT_ONCE < a.T; ++i) {
+            const unsigned t = t0 + i * kWarps * AT_ONCE + lane / SUB;
+            const float x = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
+            const float score = quantize(x, a.quantum);
+            const unsigned alive = __ballot_sync(0xffffffffu, e < a.E);
+            const unsigned first = scan_best<SUB>(score, lane, alive, a.tie_eps);
+            const unsigned rest = alive & ~__ballot_sync(0xffffffffu, e == first);
+            const unsigned second = scan_best<SUB>(score, lane, rest, a.tie_eps);
+            const unsigned lo = min(first, second), hi = max(first, second);
+            const float x0 = __shfl_sync(0xffffffffu, x, lane / SUB * SUB + lo);
+            const float x1 = __shfl_sync(0xffffffffu, x, lane / SUB * SUB + hi);
+            if (e == 0 && t < a.T) {
+                float g0 = 0.5f, g1 = 0.5f;
+                if (a.gates == B2_GATES_SOFTMAX) {
+                    const float m = fmaxf(x0, x1), p0 = expf(x0 - m), p1 = expf(x1 - m);
+                    g0 = p0 / (p0 + p1);
+                    g1 = p1 / (p0 + p1);
+                }
+                p.pair[t] = static_cast<unsigned short>(lo | hi << 8);
+                p.gate[2 * t] = g0;
+                p.gate[2 * t + 1] = g1;
+                atomicOr(&p.mask[t / 32][lo], 1u << (t & 31));
+                atomicOr(&p.mask[t / 32][hi], 1u << (t & 31));
+            }
+        }
+    }
+}
+
+// Routes the tokens and cuts every expert's into groups of CHUNK. Ends with a
+// barrier.
 template <unsigned CHUNK>
 __device__ __forceinline__ void make_plan(const MoeDecodeArgs& a, Plan& p) {
     const unsigned t = threadIdx.x, lane = t & 31, warp = t / 32;
-    const unsigned words = (a.T + 31) / 32;
-    unsigned lo = 0xFFu, hi = 0xFFu;
-    if (warp < words) {
-        if (t < a.T) {
-            float sc[kMaxExperts];
-            const float* row = a.logits + static_cast<std::size_t>(t) * a.E;
-            load_scores(row, a.E, sc);
-            const unsigned pair = top2_of_scores(sc, a.E, a.quantum, a.tie_eps);
-            lo = min(pair & 0xFFu, pair >> 8);
-            hi = max(pair & 0xFFu, pair >> 8);
-            float g0 = 0.5f, g1 = 0.5f;
-            if (a.gates == B2_GATES_SOFTMAX) {
-                const float x0 = __ldg(row + lo), x1 = __ldg(row + hi), m = fmaxf(x0, x1);
-                const float p0 = expf(x0 - m), p1 = expf(x1 - m);
-                g0 = p0 / (p0 + p1);
-                g1 = p1 / (p0 + p1);
-            }
-            p.gate[2 * t] = g0;
-            p.gate[2 * t + 1] = g1;
-        }
-        unsigned mine = 0;
-        for (unsigned e = 0; e < a.E; ++e) {
-            const unsigned m = __ballot_sync(0xffffffffu, lo == e || hi == e);
-            if (lane == e) mine = m;
-        }
-        p.mask[warp][lane] = mine;
-    }
+    if (warp < kMaxDecodeTokens / 32) p.mask[warp][lane] = 0;
     __syncthreads();
-    if (t < a.T) {
-        const unsigned below = (1u << lane) - 1u;
-        unsigned r0 = __popc(p.mask[warp][lo] & below), r1 = __popc(p.mask[warp][hi] & below);
-        for (unsigned w = 0; w < warp; ++w) {
-            r0 += __popc(p.mask[w][lo]);
-            r1 += __popc(p.mask[w][hi]);
-        }
-        p.lists[lo][r0] = static_cast<unsigned char>(2 * t);
-        p.lists[hi][r1] = static_cast<unsigned char>(2 * t + 1);
+    if (a.E <= 16) pick_experts<16>(a, p);
+    else pick_experts<32>(a, p);
+    __syncthreads();
+    if (t < 2 * a.T) {  // assignment t
+        const unsigned token = t / 2, e = t % 2 ? p.pair[token] >> 8 : p.pair[token] & 0xFFu;
+        unsigned rank = __popc(p.mask[token / 32][e] & ((1u << (token & 31)) - 1u));
+        for (unsigned w = 0; w < token / 32; ++w) rank += __popc(p.mask[w][e]);
+        p.lists[e][rank] = static_cast<unsigned char>(t);
     }
-    if (warp == 7) {
+    if (warp == kWarps - 1) {
         unsigned n = 0;
-        for (unsigned w = 0; w < words; ++w) n += __popc(p.mask[w][lane]);
+#pragma unroll
+        for (unsigned w = 0; w < kMaxDecodeTokens / 32; ++w) n += __popc(p.mask[w][lane]);
         const unsigned chunks = (n + CHUNK - 1) / CHUNK;
         unsigned end = chunks;
 #pragma unroll
@@ -184,19 +221,40 @@ constexpr unsigned kBlock = 4 * kPer<W>;
 // Parts of an activation that meet a weight.
 template <typename X, typename W>
 constexpr unsigned kParts = sizeof(X) == 2 ? 1 : sizeof(W) == 2 ? 3 : 2;
+// Activations as launch 1 leaves them for launch 2: kParts<float, W> planes.
+template <typename W>
+struct Planes {};
+template <typename X, typename W>
+struct ActOf {  // raw: one place of PER elements
+    using type = X;
+    static constexpr unsigned planes = 0;
+};
+template <typename W>
+struct ActOf<Planes<W>, W> {
+    using type = W;  // bf16 parts or TF32 parts
+    static constexpr unsigned planes = kParts<float, W>;
+};
+
+// w = hi + lo in TF32, hi rounded to nearest.
+__device__ __forceinline__ void split_tf32(unsigned w, unsigned& hi, unsigned& lo) {
+    hi = (w + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(__uint_as_float(w) - __uint_as_float(hi));
+}
 
 // The stages of one warp: MT 16-row tiles of a weight block (lane's rows r and
 // r + 8 of each) and NT 8-token tiles of activations (lane's token r), each
 // lane's bytes at its own place. VEC: every 16 bytes of a row of weights (XVEC:
 // the activations that meet them) are aligned, and inside the row or past it.
-template <typename X, typename W, unsigned MT, unsigned NT, unsigned RING, bool VEC, bool XVEC>
+template <typename A, typename W, unsigned MT, unsigned NT, bool VEC, bool XVEC>
 struct Ring {
+    using X = typename ActOf<A, W>::type;
+    static constexpr unsigned PLANES = ActOf<A, W>::planes;
     static constexpr unsigned PER = kPer<W>, BLOCK = kBlock<W>;
-    static constexpr unsigned XB = PER * sizeof(X);  // bytes of a token per lane: 32, 16 or 8
+    static constexpr unsigned XB = PLANES ? PLANES * 16 : PER * sizeof(X);  // bytes of a token per lane
     static constexpr unsigned WEIGHTS = MT * 2 * 512, STAGE = WEIGHTS + NT * 32 * XB;
-    static constexpr unsigned STAGES = RING / STAGE < 6 ? RING / STAGE : 6;
+    static constexpr unsigned STAGES = kRing / STAGE < 6 ? kRing / STAGE : 6;
     static_assert(STAGES >= 2, "a ring of one stage");
-    unsigned char* raw;     // the lane's place in the warp's first stage
+    unsigned char* raw;       // the lane's place in the warp's first stage
     unsigned base, get, put;  // shared addresses of the lane's place: first stage, next to use, next to fill
 
     __device__ __forceinline__ void init(unsigned char* warp_base, unsigned lane) {
@@ -229,23 +287,26 @@ struct Ring {
                 }
             }
     }
-    // x[n]: the lane's activations of token tile n, null where there is no
-    // token (its place is left as it is: a column nobody reads).
-    __device__ __forceinline__ void put_acts(const X* const (&x)[NT], int left, unsigned lane) {
+    // x[n]: the lane's activations of token tile n (of the first plane), null
+    // where there is no token (its place is left as it is: a column nobody
+    // reads).
+    __device__ __forceinline__ void put_acts(const X* const (&x)[NT], int left, unsigned lane, std::size_t plane) {
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
             if (!x[n]) continue;
             const unsigned at = put + WEIGHTS + n * 32 * XB;
             if (XVEC) {
-                const bool have = left > 0;
-                const X* src = x[n];  // not read where there is none
-                if constexpr (XB == 32) {
-                    copy_async_l1(at, src, have);
-                    copy_async_l1(at + 512, src + 4, have);
+                const bool have = left > 0;  // x[n] is not read where there is none
+                if constexpr (PLANES > 0) {
+#pragma unroll
+                    for (unsigned q = 0; q < PLANES; ++q) copy_async<16>(at + q * 512, x[n] + q * plane, have);
+                } else if constexpr (XB == 32) {
+                    copy_async_l1(at, x[n], have);
+                    copy_async_l1(at + 512, x[n] + 4, have);
                 } else if constexpr (XB == 16) {
-                    copy_async<16>(at, src, have);
+                    copy_async<16>(at, x[n], have);
                 } else {
-                    copy_async<8>(at - lane * 8, src, have);
+                    copy_async<8>(at - lane * 8, x[n], have);
                 }
             } else {
                 constexpr unsigned PIECE = XB >= 16 ? 16 / sizeof(X) : PER;  // elements per place
@@ -261,7 +322,7 @@ struct Ring {
 
     // part[n] += the stage's products for nt token tiles.
     __device__ __forceinline__ void multiply(unsigned nt, float (&part)[NT][MT][4], unsigned lane) {
-        constexpr unsigned PARTS = kParts<X, W>;
+        constexpr unsigned PARTS = PLANES ? PLANES : kParts<X, W>;
         uint4 w[MT][2];
 #pragma unroll
         for (unsigned m = 0; m < MT; ++m) {
@@ -273,7 +334,13 @@ struct Ring {
             if (n >= nt) break;
             const unsigned at = get + WEIGHTS + n * 32 * XB;
             unsigned b[PARTS][4];
-            if constexpr (sizeof(X) == 4 && sizeof(W) == 2) {  // x = three bf16 parts
+            if constexpr (PLANES > 0 || (sizeof(X) == 2 && sizeof(W) == 2)) {  // in parts as it lies
+#pragma unroll
+                for (unsigned q = 0; q < PARTS; ++q) {
+                    const uint4 v = lds16(at + q * 512);
+                    b[q][0] = v.x; b[q][1] = v.y; b[q][2] = v.z; b[q][3] = v.w;
+                }
+            } else if constexpr (sizeof(W) == 2) {  // x = three bf16 parts
                 const uint4 lo = lds16(at), hi = lds16(at + 512);
                 const unsigned v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -288,15 +355,12 @@ struct Ring {
                                           f2_pack(-1.0f, -1.0f), rest);
                     }
                 }
-            } else if constexpr (sizeof(W) == 2) {
-                const uint4 v = lds16(at);
-                b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
             } else if constexpr (sizeof(X) == 4) {  // x = TF32 hi + lo
                 const uint4 v = lds16(at);
-                split_tf32(v.x, b[0][0], b[1][0]);
-                split_tf32(v.y, b[0][1], b[1][1]);
-                split_tf32(v.z, b[0][2], b[1][2]);
-                split_tf32(v.w, b[0][3], b[1][3]);
+                split_tf32(v.x, b[0][0], b[PARTS - 1][0]);
+                split_tf32(v.y, b[0][1], b[PARTS - 1][1]);
+                split_tf32(v.z, b[0][2], b[PARTS - 1][2]);
+                split_tf32(v.w, b[0][3], b[PARTS - 1][3]);
             } else {
                 const uint2 v = lds8(at - lane * 8);
                 b[0][0] = v.x << 16; b[0][1] = v.x & 0xFFFF0000u;
@@ -332,11 +396,6 @@ struct Ring {
             }
         }
     }
-    // w = hi + lo in TF32, hi rounded to nearest.
-    static __device__ __forceinline__ void split_tf32(unsigned w, unsigned& hi, unsigned& lo) {
-        hi = (w + 0x1000u) & 0xFFFFE000u;
-        lo = __float_as_uint(__uint_as_float(w) - __uint_as_float(hi));
-    }
 };
 
 template <unsigned NT, unsigned MT>
@@ -360,22 +419,22 @@ __device__ __forceinline__ void flush(float (&acc)[NT][MT][4], float (&part)[NT]
 
 // ---- launch 1 ---------------------------------------------------------------------------
 
-// Item j: group j / tiles, rows j % tiles * 8 MT ... of its gate and up.
-template <typename X, typename W, unsigned MT, unsigned NT, unsigned WARPS, bool VEC>
+// Item j: group j / tiles, rows j % tiles * 8 ... of its gate and up.
+template <typename X, typename W, unsigned NT, bool VEC>
 struct Up {
-    using R = Ring<X, W, MT, NT, kUpRing, VEC, VEC>;
+    using R = Ring<X, W, 1, NT, VEC, VEC>;
     static constexpr unsigned CHUNK = 8 * NT;
     struct Smem {
-        alignas(16) unsigned char ring[WARPS][kUpRing];
-        float sums[2][WARPS][MT * 16][CHUNK + 1];  // of items j and j + 1
+        alignas(16) unsigned char ring[kWarps][kRing];
+        float sums[2][kWarps][16][CHUNK + 1];  // of items j and j + 1
         Plan plan;
     };
 };
 
-template <typename X, typename W, unsigned MT, unsigned NT, unsigned WARPS, bool VEC>
-__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS)
+template <typename X, typename W, unsigned NT, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32, 1)
 moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
-    using U = Up<X, W, MT, NT, WARPS, VEC>;
+    using U = Up<X, W, NT, VEC>;
     using R = typename U::R;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     typename U::Smem& sm = *reinterpret_cast<typename U::Smem*>(smem_raw);
@@ -389,27 +448,22 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     if (blockIdx.x >= ctas) return;
 
     const unsigned blocks = (a.H + R::BLOCK - 1) / R::BLOCK;
-    const unsigned count = blocks > warp ? (blocks - warp + WARPS - 1) / WARPS : 0u;  // per item
+    const unsigned count = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0u;  // per item
     R ring;
     ring.init(sm.ring[warp], lane);
     // the end that fills
     unsigned put_item = blockIdx.x, put_left = 0, ok = 0;
     int left = 0;
-    const W* w[MT][2] = {};
+    const W* w[1][2] = {};
     const X* x[NT] = {};
     const auto put_step = [&]() {
         if (put_left == 0) {
             if (put_item >= items || count == 0) return;
-            const unsigned g = sm.plan.group[put_item / tiles], i0 = put_item % tiles * 8 * MT;
+            const unsigned g = sm.plan.group[put_item / tiles], i = put_item % tiles * 8 + r;
             const unsigned e = group_expert(g), k = warp * R::BLOCK + c * R::PER;
-            ok = 0;
-#pragma unroll
-            for (unsigned m = 0; m < MT; ++m) {
-                const unsigned i = i0 + m * 8 + r;
-                if (i < a.I) ok |= 3u << (2 * m);
-                w[m][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H + k;
-                w[m][1] = w[m][0] + static_cast<std::size_t>(a.I) * a.H;
-            }
+            ok = i < a.I ? 3u : 0u;
+            w[0][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H + k;
+            w[0][1] = w[0][0] + static_cast<std::size_t>(a.I) * a.H;
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
                 x[t] = t * 8 + r < group_count(g)
@@ -420,29 +474,26 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             put_item += ctas;
         }
         ring.put_weights(w, ok, left, a.w_gate_up);
-        ring.put_acts(x, left, lane);
+        ring.put_acts(x, left, lane, 0);
         R::step(ring.put, ring.base);
-#pragma unroll
-        for (unsigned m = 0; m < MT; ++m) {
-            w[m][0] += WARPS * R::BLOCK;
-            w[m][1] += WARPS * R::BLOCK;
-        }
+        w[0][0] += kWarps * R::BLOCK;
+        w[0][1] += kWarps * R::BLOCK;
 #pragma unroll
         for (unsigned t = 0; t < NT; ++t)
-            if (x[t]) x[t] += WARPS * R::BLOCK;
-        left -= static_cast<int>(WARPS * R::BLOCK);
+            if (x[t]) x[t] += kWarps * R::BLOCK;
+        left -= static_cast<int>(kWarps * R::BLOCK);
         --put_left;
     };
-#pragma unroll
+#pragma unroll 1
     for (unsigned i = 0; i < R::STAGES - 1; ++i) {
         put_step();
         cp_async_commit();
     }
     unsigned buffer = 0;
     for (unsigned item = blockIdx.x; item < items; item += ctas, buffer ^= 1) {
-        const unsigned g = sm.plan.group[item / tiles], i0 = item % tiles * 8 * MT;
+        const unsigned g = sm.plan.group[item / tiles], i0 = item % tiles * 8;
         const unsigned e = group_expert(g), n = group_count(g), nt = (n + 7) / 8;
-        float acc[NT][MT][4], part[NT][MT][4];
+        float acc[NT][1][4], part[NT][1][4];
         clear(acc);
         clear(part);
         for (unsigned i = 0; i < count; ++i) {
@@ -459,46 +510,56 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
         for (unsigned t = 0; t < NT; ++t)
             if (t < nt)
 #pragma unroll
-                for (unsigned m = 0; m < MT; ++m)
-#pragma unroll
-                    for (unsigned i = 0; i < 4; ++i)
-                        sums[warp][m * 16 + r + i / 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][m][i];
+                for (unsigned i = 0; i < 4; ++i) sums[warp][r + i / 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][0][i];
         __syncthreads();  // also: everyone has read the other buffer
-        for (unsigned i = threadIdx.x; i < n * 8 * MT; i += WARPS * 32) {
-            const unsigned row = i % (8 * MT), t = i / (8 * MT), at = row / 8 * 16 + row % 8;
-            if (i0 + row >= a.act_ld) continue;
+        const unsigned row = threadIdx.x % 8, t = threadIdx.x / 8;
+        if (t < n && i0 + row < a.act_ld) {
             float gate = 0.0f, up = 0.0f;
 #pragma unroll
-            for (unsigned v = 0; v < WARPS; ++v) {
-                gate += sums[v][at][t];
-                up += sums[v][at + 8][t];
+            for (unsigned v = 0; v < kWarps; ++v) {
+                gate += sums[v][row][t];
+                up += sums[v][row + 8][t];
             }
             const unsigned to = sm.plan.lists[e][group_first(g) + t];
-            a.act[static_cast<std::size_t>(to) * a.act_ld + i0 + row] =
-                i0 + row < a.I ? gate / (1.0f + expf(-gate)) * up : 0.0f;
+            const std::size_t at = static_cast<std::size_t>(to) * a.act_ld + i0 + row;
+            const std::size_t plane = static_cast<std::size_t>(2) * a.T * a.act_ld;
+            float v = i0 + row < a.I ? gate / (1.0f + expf(-gate)) * up : 0.0f;
+            if constexpr (sizeof(W) == 2) {
+                __nv_bfloat16* act = static_cast<__nv_bfloat16*>(a.act);
+#pragma unroll
+                for (unsigned q = 0; q < 3; ++q) {
+                    const __nv_bfloat16 b = __float2bfloat16_rn(v);
+                    act[q * plane + at] = b;
+                    v -= __bfloat162float(b);
+                }
+            } else {
+                unsigned hi, lo;
+                split_tf32(__float_as_uint(v), hi, lo);
+                static_cast<unsigned*>(a.act)[at] = hi;
+                static_cast<unsigned*>(a.act)[plane + at] = lo;
+            }
         }
     }
 }
 
 // ---- launch 2 ---------------------------------------------------------------------------
 
-template <typename W, unsigned NT, bool VEC>
+template <typename W, unsigned MT, bool VEC>
 struct Down {
-    static constexpr unsigned WARPS = 8, CHUNK = 8 * NT;
-    using R = Ring<float, W, 1, NT, kDownRing, VEC, true>;
+    using R = Ring<Planes<W>, W, MT, 1, VEC, true>;
     struct Smem {
-        alignas(16) unsigned char ring[WARPS][kDownRing];
-        float sums[kDownPartials][17];
+        alignas(16) unsigned char ring[kWarps][kRing];
+        float sums[kDownPartials][16 * MT + 1];
         Plan plan;
     };
 };
 
-template <typename X, typename W, unsigned NT, bool VEC>
-__global__ void __launch_bounds__(256, 2)
+template <typename X, typename W, unsigned MT, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32, 1)
 moe_down(MoeDecodeArgs a) {
-    using D = Down<W, NT, VEC>;
+    using D = Down<W, MT, VEC>;
     using R = typename D::R;
-    constexpr unsigned WARPS = D::WARPS;
+    using Act = typename R::X;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     typename D::Smem& sm = *reinterpret_cast<typename D::Smem*>(smem_raw);
     // No wait yet: what is read up to it -- logits and weights -- was written
@@ -506,98 +567,104 @@ moe_down(MoeDecodeArgs a) {
     // launch start.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
-    make_plan<D::CHUNK>(a, sm.plan);
+    make_plan<8>(a, sm.plan);
     // k is cut in 2^shift parts so that the warps' loads even out: the fewest
     // rounds of (a part's blocks + 4, what a unit costs besides)
     const unsigned groups = sm.plan.groups, blocks = (a.I + R::BLOCK - 1) / R::BLOCK;
     unsigned shift = 0, best = ~0u;
 #pragma unroll
     for (unsigned s = 0; s < 4; ++s) {
-        const unsigned cost = (((groups << s) + WARPS - 1) / WARPS) * (((blocks + (1u << s) - 1) >> s) + 4);
+        const unsigned cost = (((groups << s) + kWarps - 1) / kWarps) * (((blocks + (1u << s) - 1) >> s) + 4);
         if (((2 * a.T) << s) <= kDownPartials && (1u << s) <= blocks && cost < best) {
             best = cost;
             shift = s;
         }
     }
-    const unsigned parts = 1u << shift, units = groups << shift, h0 = blockIdx.x * 16;
+    const unsigned parts = 1u << shift, units = groups << shift, h0 = blockIdx.x * 16 * MT;
     const auto blocks_of = [&](unsigned u) { return (blocks - (u & (parts - 1)) + parts - 1) >> shift; };
+    const std::size_t plane = static_cast<std::size_t>(2) * a.T * a.act_ld;
     R ring;
     ring.init(sm.ring[warp], lane);
 
-    // The warp's blocks are those of its units u = warp, warp + WARPS, ...,
+    // The warp's blocks are those of its units u = warp, warp + kWarps, ...,
     // one after the other through the ring.
     unsigned put_u = warp, put_left = 0, ok = 0;
     int left = 0;
-    const W* w[1][2] = {};
-    const float* x[NT] = {};
+    const W* w[MT][2] = {};
+    const Act* x[1] = {};
     const auto put_step = [&](bool with_weights, bool with_acts) {
         if (put_left == 0) {
             if (put_u >= units) return;
             const unsigned g = sm.plan.group[put_u >> shift], e = group_expert(g);
             const unsigned k = (put_u & (parts - 1)) * R::BLOCK + c * R::PER;
-            const unsigned h = h0 + r;
-            w[0][0] = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I + k;
-            w[0][1] = w[0][0] + static_cast<std::size_t>(8) * a.I;
-            ok = (h < a.H ? 1u : 0u) | (h + 8 < a.H ? 2u : 0u);
+            ok = 0;
 #pragma unroll
-            for (unsigned t = 0; t < NT; ++t)
-                x[t] = t * 8 + r < group_count(g)
-                           ? a.act + static_cast<std::size_t>(sm.plan.lists[e][group_first(g) + t * 8 + r]) * a.act_ld + k
-                           : nullptr;
+            for (unsigned i = 0; i < 2 * MT; ++i) {
+                const unsigned h = h0 + r + 8 * i;
+                w[i / 2][i % 2] = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I + k;
+                if (h < a.H) ok |= 1u << i;
+            }
+            x[0] = r < group_count(g) ? static_cast<const Act*>(a.act) +
+                                            static_cast<std::size_t>(sm.plan.lists[e][group_first(g) + r]) * a.act_ld + k
+                                      : nullptr;
             left = static_cast<int>(a.I) - static_cast<int>(k);
             put_left = blocks_of(put_u);
-            put_u += WARPS;
+            put_u += kWarps;
         }
         if (with_weights) ring.put_weights(w, ok, left, a.w_down);
         // past I the row is padded with zeros to act_ld
-        if (with_acts) ring.put_acts(x, static_cast<int>(a.act_ld) - static_cast<int>(a.I) + left, lane);
+        if (with_acts) ring.put_acts(x, static_cast<int>(a.act_ld - a.I) + left, lane, plane);
         R::step(ring.put, ring.base);
-        w[0][0] += parts * R::BLOCK;
-        w[0][1] += parts * R::BLOCK;
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t)
-            if (x[t]) x[t] += parts * R::BLOCK;
+        for (unsigned i = 0; i < 2 * MT; ++i) w[i / 2][i % 2] += parts * R::BLOCK;
+        if (x[0]) x[0] += parts * R::BLOCK;
         left -= static_cast<int>(parts * R::BLOCK);
         --put_left;
     };
     // weights of the first stages, then launch 1's activations
-    for (unsigned i = 0; i < R::STAGES - 1; ++i) put_step(true, false);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    put_u = warp;
-    put_left = 0;
-    ring.put = ring.base;
-    for (unsigned i = 0; i < R::STAGES - 1; ++i) {
-        put_step(false, true);
-        cp_async_commit();
+    bool first = true;
+#pragma unroll 1
+    for (unsigned i = 0; i < 2 * (R::STAGES - 1); ++i) {
+        if (i == R::STAGES - 1) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            put_u = warp;
+            put_left = 0;
+            ring.put = ring.base;
+            first = false;
+        }
+        put_step(first, !first);
+        if (!first) cp_async_commit();
     }
-    for (unsigned u = warp; u < units; u += WARPS) {
-        const unsigned g = sm.plan.group[u >> shift], n = group_count(g), nt = (n + 7) / 8;
+    for (unsigned u = warp; u < units; u += kWarps) {
+        const unsigned g = sm.plan.group[u >> shift], n = group_count(g);
         const unsigned count = blocks_of(u);
-        float acc[NT][1][4], part[NT][1][4];
+        float acc[1][MT][4], part[1][MT][4];
         clear(acc);
         clear(part);
         for (unsigned b = 0; b < count; ++b) {
             put_step(true, true);
             cp_async_commit();
             cp_async_wait<R::STAGES - 1>();
-            ring.multiply(nt, part, lane);
+            ring.multiply(1, part, lane);
             R::step(ring.get, ring.base);
             if (b % kChain == kChain - 1) flush(acc, part);
         }
         flush(acc, part);
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t)
+        for (unsigned e = 0; e < 2; ++e)
+            if (2 * c + e < n) {
+                float* sums = sm.sums[(u & (parts - 1)) * 2 * a.T +
+                                      sm.plan.lists[group_expert(g)][group_first(g) + 2 * c + e]];
 #pragma unroll
-            for (unsigned i = 0; i < 4; ++i) {
-                const unsigned j = t * 8 + 2 * c + i % 2;
-                if (j < n)
-                    sm.sums[(u & (parts - 1)) * 2 * a.T + sm.plan.lists[group_expert(g)][group_first(g) + j]]
-                           [r + i / 2 * 8] = acc[t][0][i];
+                for (unsigned m = 0; m < MT; ++m) {
+                    sums[m * 16 + r] = acc[0][m][e];
+                    sums[m * 16 + r + 8] = acc[0][m][2 + e];
+                }
             }
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < a.T * 16; i += WARPS * 32) {
-        const unsigned t = i / 16, h = i % 16;
+    for (unsigned i = threadIdx.x; i < a.T * 16 * MT; i += kWarps * 32) {
+        const unsigned t = i / (16 * MT), h = i % (16 * MT);
         if (h0 + h >= a.H) continue;
         float y[2] = {0.0f, 0.0f};
         for (unsigned p = 0; p < parts; ++p) {
@@ -611,32 +678,42 @@ moe_down(MoeDecodeArgs a) {
     }
 }
 
-template <typename X, typename W, unsigned MT, unsigned NT, unsigned WARPS, bool VEC>
-cudaError_t launch_tiled(const MoeDecodeArgs& a, cudaStream_t s) {
-    const unsigned tiles = (a.I + 8 * MT - 1) / (8 * MT), chunk = 8 * NT;
+template <typename X, typename W, unsigned NT, bool VEC>
+cudaError_t launch_up(const MoeDecodeArgs& a, cudaStream_t s) {
+    const unsigned tiles = (a.I + 7) / 8, chunk = 8 * NT;
     // an expert's last group may be partial, the others hold `chunk` assignments
     const unsigned groups = std::min(2 * a.T, std::min(a.E, 2 * a.T) + 2 * a.T / chunk);
-    const unsigned slots = static_cast<unsigned>(sm_count()) * (16 / WARPS);
-    const auto up = moe_gate_up<X, W, MT, NT, WARPS, VEC>;
-    const auto down = moe_down<X, W, NT, VEC>;
-    const std::size_t up_smem = sizeof(typename Up<X, W, MT, NT, WARPS, VEC>::Smem);
-    const std::size_t down_smem = sizeof(typename Down<W, NT, VEC>::Smem);
-    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(up), up_smem);
-    if (e == cudaSuccess) e = allow_dynamic_smem(reinterpret_cast<const void*>(down), down_smem);
-    if (e == cudaSuccess) e = launch_pdl(up, std::min(groups * tiles, slots), WARPS * 32, up_smem, s, a, tiles);
-    if (e == cudaSuccess) e = launch_pdl(down, (a.H + 15) / 16, 256, down_smem, s, a);
-    return e;
+    const auto kernel = moe_gate_up<X, W, NT, VEC>;
+    const std::size_t smem = sizeof(typename Up<X, W, NT, VEC>::Smem);
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, std::min(groups * tiles, static_cast<unsigned>(sm_count())), kWarps * 32, smem, s, a, tiles);
+}
+
+template <typename X, typename W, unsigned MT, bool VEC>
+cudaError_t launch_down(const MoeDecodeArgs& a, cudaStream_t s) {
+    const auto kernel = moe_down<X, W, MT, VEC>;
+    const std::size_t smem = sizeof(typename Down<W, MT, VEC>::Smem);
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, (a.H + 16 * MT - 1) / (16 * MT), kWarps * 32, smem, s, a);
 }
 
 template <typename X, typename W>
 cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
     const bool vec = a.H % 8 == 0 && a.I % kPer<W> == 0 && a.ld_x % 8 == 0 && aligned16(a.x) &&
                      aligned16(a.w_gate_up) && aligned16(a.w_down);
-    // up to 8 tokens: one 8-token tile holds any expert's, and the finest row
-    // tiles and k slices give the few experts' rows to the most warps
-    if (!vec) return launch_tiled<X, W, 2, 2, 8, false>(a, s);
-    if (a.T <= 8) return launch_tiled<X, W, 1, 1, 16, true>(a, s);
-    return launch_tiled<X, W, 2, 2, 8, true>(a, s);
+    // 16 tokens per group where the experts have more than 4 on average: fewer
+    // experts are read twice; else 8, whose smaller stages leave more weights in flight
+    const bool wide = 2 * a.T > 4 * a.E;
+    cudaError_t e = !vec   ? launch_up<X, W, 2, false>(a, s)
+                    : wide ? launch_up<X, W, 2, true>(a, s)
+                           : launch_up<X, W, 1, true>(a, s);
+    if (e != cudaSuccess) return e;
+    // 32 output rows per CTA as long as that reaches most SMs: the activations are read once for both tiles
+    const bool tall = a.H >= 2368;
+    if (vec) return tall ? launch_down<X, W, 2, true>(a, s) : launch_down<X, W, 1, true>(a, s);
+    return tall ? launch_down<X, W, 2, false>(a, s) : launch_down<X, W, 1, false>(a, s);
 }
 
 }  // namespace
@@ -649,7 +726,7 @@ int b2_moe_decode_workspace_size(size_t T, size_t I, size_t* bytes) {
     if (!bytes) return invalid("b2_moe_decode_workspace_size: null pointer");
     if (T > kMaxDecodeTokens || I > 0x7FFFFFFu)
         return invalid("b2_moe_decode_workspace_size: T must be 128 at most, I below 2^27");
-    *bytes = 2 * T * ((I + 7) / 8 * 8) * sizeof(float) + 16;
+    *bytes = 2 * T * ((I + 7) / 8 * 8) * 8 + 16;  // up to two fp32 parts
     return B2_OK;
 }
 
@@ -677,7 +754,7 @@ int b2_moe_decode(const void* x, size_t ld_x, uint32_t x_dtype, const float* log
     a.E = static_cast<unsigned>(E); a.I = static_cast<unsigned>(I);
     a.quantum = quantum; a.tie_eps = tie_eps; a.gates = gates;
     a.w_gate_up = w_gate_up; a.w_down = w_down; a.out = out; a.ld_out = ld_out;
-    a.act = static_cast<float*>(workspace);
+    a.act = workspace;
     a.act_ld = static_cast<unsigned>((I + 7) / 8 * 8);
     cudaStream_t s = as_stream(stream);
     cudaError_t e;
