@@ -986,29 +986,30 @@ __device__ __forceinline__ void join_parts(const AttnKv4Args& a, const Tile& t, 
         }
         return;
     }
-    float* factor = reinterpret_cast<float*>(sm.ring);  // [rows][n]
+    // References and sums first, then all parts' sums, cut among the threads
+    // that a row's outputs leave idle, each cut added in order.
+    float2* factor = reinterpret_cast<float2*>(sm.ring);  // [rows][n]
     if (warp < t.rows) {
+        float2* mine = factor + warp * n;
         float m = kNegInf, l = 0.0f;
         for (unsigned i = lane; i < n; i += 32) {
-            const float x = __ldcg(&refs[slot(i) * kRows + warp].x);
-            factor[warp * n + i] = x;
-            m = fmaxf(m, x);
+            const float2 v = __ldcg(refs + slot(i) * kRows + warp);
+            mine[i] = v;
+            m = fmaxf(m, v.x);
         }
         m = warp_max(m);
         for (unsigned i = lane; i < n; i += 32) {
-            const float ref = factor[warp * n + i];
-            const float w = ref == kNegInf ? 0.0f : exp2_approx(ref - m);
-            factor[warp * n + i] = w;
-            l += w * __ldcg(&refs[slot(i) * kRows + warp].y);
+            const float w = mine[i].x == kNegInf ? 0.0f : exp2_approx(mine[i].x - m);
+            l = fmaf(w, mine[i].y, l);
+            mine[i].x = w;
         }
         l = warp_sum(l);
         if (lane == 0) sm.row_sum[warp] = l;
     }
     __syncthreads();
-    // the parts are cut among the threads that a row's outputs leave idle, and added in order
     const unsigned outputs = t.rows * (D / 4);
     const unsigned cuts = max(1u, min(kWarps * 32 / outputs, 8u)), per = (n + cuts - 1) / cuts;
-    float4* sums = reinterpret_cast<float4*>(sm.ring) + (kRows * kMaxGrid) / 4;  // [cuts][outputs]
+    float4* sums = reinterpret_cast<float4*>(sm.ring) + kRows * kMaxGrid / 2;  // [cuts][outputs]
     for (unsigned i = threadIdx.x; i < outputs * cuts; i += kWarps * 32) {
         const unsigned cut = i / outputs, o = i % outputs, row = o / (D / 4), d4 = o % (D / 4);
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1016,7 +1017,7 @@ __device__ __forceinline__ void join_parts(const AttnKv4Args& a, const Tile& t, 
 #pragma unroll 10
         for (unsigned k = cut * per; k < end; ++k) {
             const float4 v = __ldcg(parts + (slot(k) * kRows + row) * (D / 4) + d4);
-            const float w = factor[row * n + k];
+            const float w = factor[row * n + k].x;
             if (w != 0.0f) add(s, w, v);
         }
         sums[cut * outputs + o] = s;
@@ -1220,7 +1221,7 @@ attention_kv4_shares(AttnKv4Args a) {
     };
 
     // ---- sizes of all pairs; rows that see nothing are written here ----
-    unsigned long long all_units = 0;
+    unsigned all_units = 0;  // the entry point sees to it that sums fit 32 bits
     unsigned units = 0, before = 0, total = 0;  // of pair threadIdx.x, when there are up to kPairCache
     for (unsigned p0 = 0; p0 < pairs; p0 += kPairCache) {
         const unsigned p = p0 + threadIdx.x;
@@ -1236,23 +1237,19 @@ attention_kv4_shares(AttnKv4Args a) {
         if (scan_units(units, blank, sm, &before, &total)) write_blank_rows<T, D, Rows::ROWS>(a, p0);
         all_units += total;
     }
-    const unsigned long long work = all_units * heads;
-    unsigned long long share = (work + gridDim.x - 1) / gridDim.x;
+    const unsigned work = all_units * heads;
     // short contexts: not less than a pair, up to a unit per warp, so that a
     // pair is not cut for nothing
-    const unsigned long long per_pair = (work + static_cast<unsigned long long>(pairs) * heads - 1) /
-                                        (static_cast<unsigned long long>(pairs) * heads);
-    share = max(share, min(per_pair, static_cast<unsigned long long>(kWarps)));
+    const unsigned share = max((work + gridDim.x - 1) / gridDim.x, min((all_units + pairs - 1) / pairs, kWarps));
 
     // ---- pairs on CTAs of their own, if that leaves no CTA with much more
     // than its share: a second part costs a CTA what some 16 units do ----
     Part part;
-    unsigned long long at = 0, stop = 0;  // else: the CTA's share of the list
-    unsigned long long pair_begin = 0;    // units of earlier pairs, one head
-    unsigned block0 = 0;                  // first pair of the cached block
+    unsigned at = 0, stop = 0;    // else: the CTA's share of the list
+    unsigned pair_begin = 0;      // units of earlier pairs, one head
+    unsigned block0 = 0;          // first pair of the cached block
     unsigned most = 0;
-    if (pairs <= kPairCache && static_cast<unsigned long long>(pairs) * heads <= gridDim.x && share < 0x10000000u)
-        most = fit_pairs<D>(pairs, heads, static_cast<unsigned>(share), sm);
+    if (pairs <= kPairCache && pairs * heads <= gridDim.x) most = fit_pairs<D>(pairs, heads, share, sm);
     if (most) {
         const unsigned n = (units + most - 1) / most;  // CTAs of this thread's pair, per head
         scan_units(n, false, sm, &before, &total);
@@ -1273,9 +1270,9 @@ attention_kv4_shares(AttnKv4Args a) {
         part.to = min(all, part.from + each);
         if (index >= part.n) return;
     } else {
+        if (blockIdx.x >= (work + share - 1) / share) return;
         at = blockIdx.x * share;
         stop = min(at + share, work);
-        if (at >= stop) return;
         for (unsigned p0 = 0; p0 < pairs; p0 += kPairCache) {
             const unsigned p = p0 + threadIdx.x;
             if (pairs > kPairCache) {
@@ -1283,8 +1280,8 @@ attention_kv4_shares(AttnKv4Args a) {
                 scan_units(units, false, sm, &before, &total);
                 sm.pair_units[threadIdx.x] = units;
             }
-            const unsigned long long b = (pair_begin + before) * heads;
-            if (units && at >= b && at < b + static_cast<unsigned long long>(units) * heads) {
+            const unsigned b = (pair_begin + before) * heads;
+            if (units && at >= b && at < b + units * heads) {
                 sm.found_pair = p;
                 sm.found_before = before;
             }
@@ -1306,12 +1303,12 @@ attention_kv4_shares(AttnKv4Args a) {
                 if (at < (pair_begin + size) * heads) break;
                 pair_begin += size;
             }
-            part.head = static_cast<unsigned>((at - pair_begin * heads) / size);
-            const unsigned long long begin = pair_begin * heads + static_cast<unsigned long long>(part.head) * size;
-            part.from = static_cast<unsigned>(at - begin);
-            part.to = static_cast<unsigned>(min(begin + size, stop) - begin);
-            part.first = static_cast<unsigned>(begin / share);
-            part.n = static_cast<unsigned>((begin + size - 1) / share) - part.first + 1;
+            part.head = (at - pair_begin * heads) / size;
+            const unsigned begin = pair_begin * heads + part.head * size;
+            part.from = at - begin;
+            part.to = min(begin + size, stop) - begin;
+            part.first = begin / share;
+            part.n = (begin + size - 1) / share - part.first + 1;
             at = begin + part.to;
         }
         run_part<T, D, Rows>(a, part, sm);
@@ -1384,6 +1381,9 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride, v
     const std::size_t tiles = (max_queries * a.group + (narrow ? 3 : 7)) / (narrow ? 4 : 8);
     if (cache->seqs > 0x7FFFFFFFu / tiles) return invalid("b2_attention_kv4: too many row tiles");
     a.tiles = static_cast<unsigned>(tiles);
+    // the kernel counts steps of 32 keys, over all pairs and heads, in 32 bits
+    if ((max_len / kStep + 1) * cache->seqs > 0x3FFFFFFFu / (tiles * cache->kv_heads))
+        return invalid("b2_attention_kv4: seqs * row tiles * kv_heads * max_len past 2^35 (max_len bounds the lengths)");
     a.counters = static_cast<unsigned*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.counters + kMaxGrid);
     a.part_o = a.part_ml + 2 * kMaxGrid * kRows * 2;
