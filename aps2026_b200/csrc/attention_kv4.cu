@@ -131,7 +131,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// `bytes` of the copy are read, the rest of SIZE is zero.
+__device__ __forceinline__ void copy_async16(unsigned dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// SIZE bytes of src, or zeros.
 template <int SIZE>
 __device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool have) {
     const int bytes = have ? SIZE : 0;
@@ -193,17 +196,6 @@ __device__ __forceinline__ std::size_t row_of(const AttnKv4Args& a, const Tile& 
     return t.first_row + f / a.group;
 }
 
-// The page of this lane's position in the step from key u0; kKv4Padding when
-// there is none.
-__device__ __forceinline__ unsigned lane_page(const AttnKv4Args& a, const Tile& t, unsigned seq, unsigned u) {
-    unsigned page = kKv4Padding;
-    if (u < t.total && !kv4_page(a.cache, seq, key_position(t, u), &page)) {
-        flag_check(B2_CHECK_KV4);
-        page = kKv4Padding;
-    }
-    return page;
-}
-
 // Place of 16-byte chunk `part` of key tok's V row in a stage: swizzled inside
 // 128-byte lines, so that the 4 bytes that each of 8 x 4 lanes reads of 4
 // keys' rows hit all banks.
@@ -213,58 +205,92 @@ __device__ __forceinline__ unsigned v_offset(unsigned tok, unsigned part) {
     return line * 128 + ((at ^ ((D == 128 ? line & 3u : line & 1u) << 1)) << 4);
 }
 
-// Issues the copies of one step into `stage`; `page` is this lane's.
+// What a warp needs to bring a pair's steps into its ring.
 template <unsigned D>
-__device__ __forceinline__ void stage_step(const AttnKv4Args& a, const Tile& t, unsigned head, unsigned u0,
-                                           unsigned page, unsigned stage, unsigned* valid, unsigned lane) {
+struct Feed {
     using S = Shape<D>;
-    constexpr unsigned PARTS = D / 32;       // 16-byte chunks of a row of codes
-    constexpr unsigned COPIES = PARTS;       // chunks per lane
-    const unsigned shift = a.cache.page_shift, slots = (1u << shift) - 1u;
-    const std::uint8_t* heads = a.cache.data + head * a.cache.head_stride;
-    const unsigned part = lane % PARTS;
-    constexpr unsigned P = 4 * S::groups;
-    // keys lane / PARTS + i * (32 / PARTS): whole swizzle periods apart
-    const unsigned v_at = stage + S::codes + v_offset<D>(lane / PARTS, part);
-    const unsigned j0 = key_position(t, u0);
-    if (u0 + kStep <= t.total && (u0 >= t.sinks || u0 + kStep <= t.sinks) &&
-        ((j0 ^ (j0 + kStep - 1)) >> shift) == 0 && __any_sync(0xffffffffu, page != kKv4Padding)) {
-        // 32 neighbours of one page: four runs of memory
-        if (lane == 0) *valid = 0xFFFFFFFFu;
-        const std::uint8_t* block = heads + page * a.cache.page_stride;
-        const unsigned slot = j0 & slots;
-        const std::uint8_t* codes = block + (slot * (D / 2) + lane * 16);
-        const std::uint8_t* v_codes = codes + kv4_v_codes<D>(shift);
-#pragma unroll
-        for (unsigned i = 0; i < COPIES; ++i) {
-            copy_async<16>(stage + lane * 16 + i * 512, codes + i * 512, true);
-            copy_async<16>(v_at + i * 512, v_codes + i * 512, true);
+    static constexpr unsigned PARTS = D / 32;  // 16-byte chunks of a row of codes = copies per lane
+    static constexpr unsigned P = 4 * S::groups;
+    const std::uint8_t* head;     // the KV head's block of page 0
+    const std::uint32_t* table;   // the sequence's pages
+    unsigned lane, v_at;          // v_at: place of the lane's first V chunk in a stage
+    unsigned sinks, skip, total;  // key u is position u, past the sinks u + skip
+
+    __device__ __forceinline__ void init(const AttnKv4Args& a, const Tile& t, unsigned seq, unsigned h, unsigned lane_) {
+        head = a.cache.data + h * a.cache.head_stride;
+        table = a.cache.table + static_cast<std::size_t>(seq) * a.cache.max_pages;
+        lane = lane_;
+        // keys lane / PARTS + i * (32 / PARTS): whole swizzle periods apart
+        v_at = S::codes + v_offset<D>(lane / PARTS, lane % PARTS);
+        sinks = t.sinks;
+        skip = t.low - t.sinks;
+        total = t.total;
+    }
+    __device__ __forceinline__ unsigned position(unsigned u) const { return u < sinks ? u : u + skip; }
+    // Whether the step from key u0 is 32 neighbours of one page.
+    __device__ __forceinline__ bool one_page(const AttnKv4Args& a, unsigned u0) const {
+        const unsigned slots = (1u << a.cache.page_shift) - 1u;
+        return u0 + kStep <= total && (u0 >= sinks || u0 + kStep <= sinks) && (position(u0) & slots) + kStep - 1 <= slots;
+    }
+    // The page of this lane's key of the step from u0 (the same for all lanes
+    // of a one-page step); kKv4Padding where there is none. The length check
+    // keeps positions inside the table.
+    __device__ __forceinline__ unsigned page(const AttnKv4Args& a, unsigned u0) const {
+        const unsigned u = u0 + lane;
+        unsigned pg = kKv4Padding;
+        if (u < total) {
+            pg = __ldg(table + (position(u) >> a.cache.page_shift));
+            if (pg >= a.cache.pages) {
+                flag_check(B2_CHECK_KV4);
+                pg = kKv4Padding;
+            }
         }
-        const std::uint8_t* params = block + kv4_k_params<D>(shift) + (slot + lane) * P;
-        copy_async<P>(stage + 2 * S::codes + lane * P, params, true);
-        copy_async<P>(stage + 2 * S::codes + S::params + lane * P, params + (P << shift), true);
-        return;
+        return pg;
     }
-    const unsigned have = __ballot_sync(0xffffffffu, page != kKv4Padding);
-    if (lane == 0) *valid = have;
+    // Issues the copies of the step from u0 into `stage`; pg: page(u0).
+    __device__ __forceinline__ void copy(const AttnKv4Args& a, unsigned u0, unsigned pg, unsigned stage,
+                                         unsigned* valid) const {
+        const unsigned shift = a.cache.page_shift, slots = (1u << shift) - 1u;
+        if (one_page(a, u0) && __any_sync(0xffffffffu, pg != kKv4Padding)) {  // four runs of memory
+            if (lane == 0) *valid = 0xFFFFFFFFu;
+            const unsigned slot = position(u0) & slots;
+            const std::uint8_t* block = head + static_cast<unsigned long long>(pg) * a.cache.page_stride;
+            const std::uint8_t* codes = block + (slot * (D / 2) + lane * 16);
+            const std::uint8_t* v_codes = codes + kv4_v_codes<D>(shift);
+            const unsigned k_dst = stage + lane * 16, v_dst = stage + v_at;
 #pragma unroll
-    for (unsigned i = 0; i < COPIES; ++i) {
-        const unsigned tok = i * (32 / PARTS) + lane / PARTS;
-        const unsigned pg = __shfl_sync(0xffffffffu, page, tok);
+            for (unsigned i = 0; i < PARTS; ++i) {
+                copy_async16(k_dst + i * 512, codes + i * 512);
+                copy_async16(v_dst + i * 512, v_codes + i * 512);
+            }
+            const std::uint8_t* params = block + (kv4_k_params<D>(shift) + (slot + lane) * P);
+            copy_async<P>(stage + 2 * S::codes + lane * P, params, true);
+            copy_async<P>(stage + 2 * S::codes + S::params + lane * P, params + (P << shift), true);
+            return;
+        }
+        const unsigned have = __ballot_sync(0xffffffffu, pg != kKv4Padding);
+        if (lane == 0) *valid = have;
+        const unsigned part = lane % PARTS;
+#pragma unroll
+        for (unsigned i = 0; i < PARTS; ++i) {
+            const unsigned tok = i * (32 / PARTS) + lane / PARTS;
+            const unsigned from = __shfl_sync(0xffffffffu, pg, tok);
+            const bool ok = from != kKv4Padding;
+            const unsigned slot = position(u0 + tok) & slots;
+            const std::uint8_t* src = ok ? head + static_cast<unsigned long long>(from) * a.cache.page_stride +
+                                               (slot * (D / 2) + part * 16)
+                                         : a.cache.data;
+            copy_async<16>(stage + tok * (D / 2) + part * 16, src, ok);
+            copy_async<16>(stage + v_at + i * 512, ok ? src + kv4_v_codes<D>(shift) : src, ok);
+        }
         const bool ok = pg != kKv4Padding;
-        const unsigned slot = key_position(t, u0 + tok) & slots;
-        const std::uint8_t* src =
-            ok ? heads + pg * a.cache.page_stride + (slot * (D / 2) + part * 16) : a.cache.data;
-        copy_async<16>(stage + tok * (D / 2) + part * 16, src, ok);
-        copy_async<16>(v_at + i * 512, ok ? src + kv4_v_codes<D>(shift) : src, ok);
+        const unsigned slot = position(u0 + lane) & slots;
+        const std::uint8_t* block = ok ? head + static_cast<unsigned long long>(pg) * a.cache.page_stride : a.cache.data;
+        copy_async<P>(stage + 2 * S::codes + lane * P, block + (ok ? kv4_k_params<D>(shift) + slot * P : 0u), ok);
+        copy_async<P>(stage + 2 * S::codes + S::params + lane * P, block + (ok ? kv4_v_params<D>(shift) + slot * P : 0u),
+                      ok);
     }
-    const bool ok = page != kKv4Padding;
-    const unsigned slot = key_position(t, u0 + lane) & slots;
-    const std::uint8_t* block = ok ? heads + page * a.cache.page_stride : a.cache.data;
-    copy_async<P>(stage + 2 * S::codes + lane * P, block + (ok ? kv4_k_params<D>(shift) + slot * P : 0u), ok);
-    copy_async<P>(stage + 2 * S::codes + S::params + lane * P, block + (ok ? kv4_v_params<D>(shift) + slot * P : 0u),
-                  ok);
-}
+};
 
 // Pairs of fp32 in one register pair: two results per instruction.
 using f32x2 = unsigned long long;
@@ -1042,18 +1068,19 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
     const auto key_of = [&](unsigned i) { return (from + warp + i * kWarps) * kStep; };
     const unsigned ring = smem_addr(sm.ring[warp]);
     // page numbers, then queries, then keys: each latency starts as early as it can
+    Feed<D> feed;
+    feed.init(a, t, seq, head, lane);
     unsigned pages[S::stages], next_page = kKv4Padding;
 #pragma unroll
-    for (unsigned i = 0; i < S::stages; ++i)
-        pages[i] = i < steps ? lane_page(a, t, seq, key_of(i) + lane) : kKv4Padding;
+    for (unsigned i = 0; i < S::stages; ++i) pages[i] = i < steps ? feed.page(a, key_of(i)) : kKv4Padding;
     float query[D / 32];
     fetch_query<T, D, Rows::ROWS>(a, t, head, query);
 #pragma unroll
     for (unsigned i = 0; i < S::stages; ++i) {
-        if (i < steps) stage_step<D>(a, t, head, key_of(i), pages[i], ring + i * S::stage, &sm.valid[warp][i], lane);
+        if (i < steps) feed.copy(a, key_of(i), pages[i], ring + i * S::stage, &sm.valid[warp][i]);
         cp_async_commit();
     }
-    if (S::stages < steps) next_page = lane_page(a, t, seq, key_of(S::stages) + lane);
+    if (S::stages < steps) next_page = feed.page(a, key_of(S::stages));
     place_query<D, Rows>(a, query, sm);
     __syncthreads();  // queries
 
@@ -1068,9 +1095,8 @@ __device__ __forceinline__ void run_segment(const AttnKv4Args& a, const Tile& t,
         rows.step(a, t, sm, stage, u0, valid, clear);
         __syncwarp();
         if (i + S::stages < steps) {
-            stage_step<D>(a, t, head, key_of(i + S::stages), next_page, stage, &sm.valid[warp][at], lane);
-            next_page = i + S::stages + 1 < steps ? lane_page(a, t, seq, key_of(i + S::stages + 1) + lane)
-                                                  : kKv4Padding;
+            feed.copy(a, key_of(i + S::stages), next_page, stage, &sm.valid[warp][at]);
+            if (i + S::stages + 1 < steps) next_page = feed.page(a, key_of(i + S::stages + 1));
         }
         cp_async_commit();
     }

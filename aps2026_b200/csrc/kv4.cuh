@@ -40,7 +40,7 @@ struct Kv4View {
     std::uint8_t* data;
     const std::uint32_t* table;
     unsigned pages, page_shift, kv_heads, seqs, max_pages;
-    std::size_t head_stride, page_stride;  // bytes of a head's block, of a page
+    unsigned head_stride, page_stride;  // bytes of a head's block, of a page
 };
 
 // Sections of the block of (page, head), in bytes from its start.
@@ -54,7 +54,7 @@ __device__ __forceinline__ unsigned kv4_v_params(unsigned page_shift) {
 }
 
 __device__ __forceinline__ std::uint8_t* kv4_block(const Kv4View& c, unsigned page, unsigned head) {
-    return c.data + page * c.page_stride + head * c.head_stride;
+    return c.data + static_cast<std::size_t>(page) * c.page_stride + static_cast<std::size_t>(head) * c.head_stride;
 }
 
 // The page of position `pos` of sequence `seq`; false if the sequence, the
@@ -93,8 +93,10 @@ inline int kv4_view(const b2_kv4_cache* c, const char* what, Kv4View* view) {
     view->kv_heads = static_cast<unsigned>(c->kv_heads);
     view->seqs = static_cast<unsigned>(c->seqs);
     view->max_pages = static_cast<unsigned>(c->max_pages);
-    view->head_stride = c->page_size * (c->head_dim == 64 ? Kv4Row<64>::bytes : Kv4Row<128>::bytes);
-    view->page_stride = view->head_stride * c->kv_heads;
+    const std::size_t head_bytes = c->page_size * (c->head_dim == 64 ? Kv4Row<64>::bytes : Kv4Row<128>::bytes);
+    if (head_bytes > 0xFFFFFFFFu / c->kv_heads) return invalid(at + ": a page of 4 GB or more");
+    view->head_stride = static_cast<unsigned>(head_bytes);
+    view->page_stride = static_cast<unsigned>(head_bytes * c->kv_heads);
     return B2_OK;
 }
 
