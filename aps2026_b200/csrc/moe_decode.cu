@@ -21,7 +21,7 @@
 // after the other through the same rings. Its warps interleave the k blocks,
 // so together they read whole lines, and add up in shared memory. It leaves
 // the activations in their parts. Launch 2, moe_down: CTA = 16 MT rows of the
-// output for all tokens; warps take (expert, 8 of its tokens, part of k) and
+// output for all tokens; warps take (expert, 8 NT of its tokens, part of k) and
 // meet in shared memory, where a token's two experts are summed in ascending
 // order: no float atomics, results repeat. Each CTA routes for itself (T x E
 // logits). Launch 2 starts under launch 1 and has routed and requested its
@@ -196,6 +196,9 @@ __device__ __forceinline__ uint2 lds8(unsigned addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ void copy_async16(unsigned dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // SIZE bytes of src, or zeros.
 template <int SIZE>
 __device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool have) {
@@ -266,6 +269,34 @@ struct Ring {
         if (at == base + STAGES * STAGE) at = base;
     }
 
+    // A stage that is inside its rows for all lanes. Rows and tokens that are
+    // not there are left as they are: sums that nobody reads.
+    __device__ __forceinline__ void put_whole(const W* const (&w)[MT][2], unsigned ok, bool with_weights,
+                                              const X* const (&x)[NT], unsigned x_ok, bool with_acts, unsigned lane,
+                                              std::size_t plane) {
+        static_assert(VEC && XVEC, "aligned rows");
+        if (with_weights)
+#pragma unroll
+            for (unsigned i = 0; i < 2 * MT; ++i)
+                if ((ok >> i) & 1u) copy_async16(put + i * 512, w[i / 2][i % 2]);
+        if (with_acts)
+#pragma unroll
+            for (unsigned n = 0; n < NT; ++n)
+                if ((x_ok >> n) & 1u) {
+                    const unsigned at = put + WEIGHTS + n * 32 * XB;
+                    if constexpr (PLANES > 0) {
+#pragma unroll
+                        for (unsigned q = 0; q < PLANES; ++q) copy_async16(at + q * 512, x[n] + q * plane);
+                    } else if constexpr (XB == 32) {
+                        copy_async_l1(at, x[n], true);
+                        copy_async_l1(at + 512, x[n] + 4, true);
+                    } else if constexpr (XB == 16) {
+                        copy_async16(at, x[n]);
+                    } else {
+                        copy_async<8>(at - lane * 8, x[n], true);
+                    }
+                }
+    }
     // w[m][i]: the lane's weights (row's start + k); ok: bit 2m + i set where
     // the row is there; left: weights from k to the row's end, if positive.
     __device__ __forceinline__ void put_weights(const W* const (&w)[MT][2], unsigned ok, int left, const void* any) {
@@ -278,22 +309,37 @@ struct Ring {
                     const bool have = row && left > 0;
                     copy_async<16>(put + (m * 2 + i) * 512, have ? w[m][i] : any, have);
                 } else {
+                    unsigned char* dst = raw + (put - base) + (m * 2 + i) * 512;
+                    if (sizeof(W) == 2 && row && left > static_cast<int>(PER) && w[m][i] != any) {
+                        // 8 bf16 from the 4 (5, when they straddle) words that hold them: the
+                        // row goes on behind them, and the tensor began before them
+                        const std::uintptr_t at = reinterpret_cast<std::uintptr_t>(w[m][i]);
+                        const unsigned* words = reinterpret_cast<const unsigned*>(at & ~std::uintptr_t(3));
+                        const unsigned shift = (at & 2u) * 8;
+                        unsigned v[5];
+#pragma unroll
+                        for (unsigned e = 0; e < 4; ++e) v[e] = __ldg(words + e);
+                        v[4] = shift ? __ldg(words + 4) : 0u;
+                        *reinterpret_cast<uint4*>(dst) =
+                            make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
+                                       __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
+                        continue;
+                    }
                     W v[PER];
 #pragma unroll
                     for (unsigned e = 0; e < PER; ++e) v[e] = row && static_cast<int>(e) < left ? w[m][i][e] : W(0.0f);
-                    W* dst = reinterpret_cast<W*>(raw + (put - base) + (m * 2 + i) * 512);
 #pragma unroll
-                    for (unsigned e = 0; e < PER; ++e) dst[e] = v[e];
+                    for (unsigned e = 0; e < PER; ++e) reinterpret_cast<W*>(dst)[e] = v[e];
                 }
             }
     }
-    // x[n]: the lane's activations of token tile n (of the first plane), null
-    // where there is no token (its place is left as it is: a column nobody
-    // reads).
-    __device__ __forceinline__ void put_acts(const X* const (&x)[NT], int left, unsigned lane, std::size_t plane) {
+    // x[n]: the lane's activations of token tile n (of the first plane); x_ok:
+    // bit n set where there is a token.
+    __device__ __forceinline__ void put_acts(const X* const (&x)[NT], unsigned x_ok, int left, unsigned lane,
+                                             std::size_t plane) {
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
-            if (!x[n]) continue;
+            if (!((x_ok >> n) & 1u)) continue;
             const unsigned at = put + WEIGHTS + n * 32 * XB;
             if (XVEC) {
                 const bool have = left > 0;  // x[n] is not read where there is none
@@ -382,8 +428,12 @@ struct Ring {
                     unsigned h0[4], l0[4], h1[4], l1[4];
 #pragma unroll
                     for (unsigned i = 0; i < 4; ++i) {
-                        split_tf32(r0[i], h0[i], l0[i]);
-                        split_tf32(r1[i], h1[i], l1[i]);
+                        // hi truncated: its rounding would cost another operation
+                        // per weight; lo then has 13 bits, of which TF32 keeps 11
+                        h0[i] = r0[i] & 0xFFFFE000u;
+                        l0[i] = __float_as_uint(__uint_as_float(r0[i]) - __uint_as_float(h0[i]));
+                        h1[i] = r1[i] & 0xFFFFE000u;
+                        l1[i] = __float_as_uint(__uint_as_float(r1[i]) - __uint_as_float(h1[i]));
                     }
 #pragma unroll
                     for (unsigned i = 0; i < 4; i += 2) {
@@ -452,7 +502,7 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     R ring;
     ring.init(sm.ring[warp], lane);
     // the end that fills
-    unsigned put_item = blockIdx.x, put_left = 0, ok = 0;
+    unsigned put_item = blockIdx.x, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
     const W* w[1][2] = {};
     const X* x[NT] = {};
@@ -464,23 +514,28 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             ok = i < a.I ? 3u : 0u;
             w[0][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H + k;
             w[0][1] = w[0][0] + static_cast<std::size_t>(a.I) * a.H;
+            x_ok = 0;
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
-                x[t] = t * 8 + r < group_count(g)
-                           ? static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x + k
-                           : nullptr;
+                if (t * 8 + r < group_count(g)) {
+                    x_ok |= 1u << t;
+                    x[t] = static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x + k;
+                }
             left = static_cast<int>(a.H) - static_cast<int>(k);
             put_left = count;
             put_item += ctas;
         }
-        ring.put_weights(w, ok, left, a.w_gate_up);
-        ring.put_acts(x, left, lane, 0);
+        if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
+            if constexpr (VEC) ring.put_whole(w, ok, true, x, x_ok, true, lane, 0);
+        } else {
+            ring.put_weights(w, ok, left, a.w_gate_up);
+            ring.put_acts(x, x_ok, left, lane, 0);
+        }
         R::step(ring.put, ring.base);
         w[0][0] += kWarps * R::BLOCK;
         w[0][1] += kWarps * R::BLOCK;
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t)
-            if (x[t]) x[t] += kWarps * R::BLOCK;
+        for (unsigned t = 0; t < NT; ++t) x[t] += kWarps * R::BLOCK;
         left -= static_cast<int>(kWarps * R::BLOCK);
         --put_left;
     };
@@ -544,9 +599,9 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
 
 // ---- launch 2 ---------------------------------------------------------------------------
 
-template <typename W, unsigned MT, bool VEC>
+template <typename W, unsigned MT, unsigned NT, bool VEC>
 struct Down {
-    using R = Ring<Planes<W>, W, MT, 1, VEC, true>;
+    using R = Ring<Planes<W>, W, MT, NT, VEC, true>;
     struct Smem {
         alignas(16) unsigned char ring[kWarps][kRing];
         float sums[kDownPartials][16 * MT + 1];
@@ -554,10 +609,10 @@ struct Down {
     };
 };
 
-template <typename X, typename W, unsigned MT, bool VEC>
+template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, 1)
 moe_down(MoeDecodeArgs a) {
-    using D = Down<W, MT, VEC>;
+    using D = Down<W, MT, NT, VEC>;
     using R = typename D::R;
     using Act = typename R::X;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -567,7 +622,7 @@ moe_down(MoeDecodeArgs a) {
     // launch start.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
-    make_plan<8>(a, sm.plan);
+    make_plan<8 * NT>(a, sm.plan);
     // k is cut in 2^shift parts so that the warps' loads even out: the fewest
     // rounds of (a part's blocks + 4, what a unit costs besides)
     const unsigned groups = sm.plan.groups, blocks = (a.I + R::BLOCK - 1) / R::BLOCK;
@@ -588,10 +643,10 @@ moe_down(MoeDecodeArgs a) {
 
     // The warp's blocks are those of its units u = warp, warp + kWarps, ...,
     // one after the other through the ring.
-    unsigned put_u = warp, put_left = 0, ok = 0;
+    unsigned put_u = warp, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
     const W* w[MT][2] = {};
-    const Act* x[1] = {};
+    const Act* x[NT] = {};
     const auto put_step = [&](bool with_weights, bool with_acts) {
         if (put_left == 0) {
             if (put_u >= units) return;
@@ -604,20 +659,30 @@ moe_down(MoeDecodeArgs a) {
                 w[i / 2][i % 2] = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I + k;
                 if (h < a.H) ok |= 1u << i;
             }
-            x[0] = r < group_count(g) ? static_cast<const Act*>(a.act) +
-                                            static_cast<std::size_t>(sm.plan.lists[e][group_first(g) + r]) * a.act_ld + k
-                                      : nullptr;
+            x_ok = 0;
+#pragma unroll
+            for (unsigned t = 0; t < NT; ++t)
+                if (t * 8 + r < group_count(g)) {
+                    x_ok |= 1u << t;
+                    x[t] = static_cast<const Act*>(a.act) +
+                           static_cast<std::size_t>(sm.plan.lists[e][group_first(g) + t * 8 + r]) * a.act_ld + k;
+                }
             left = static_cast<int>(a.I) - static_cast<int>(k);
             put_left = blocks_of(put_u);
             put_u += kWarps;
         }
-        if (with_weights) ring.put_weights(w, ok, left, a.w_down);
-        // past I the row is padded with zeros to act_ld
-        if (with_acts) ring.put_acts(x, static_cast<int>(a.act_ld - a.I) + left, lane, plane);
+        if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
+            if constexpr (VEC) ring.put_whole(w, ok, with_weights, x, x_ok, with_acts, lane, plane);
+        } else {
+            if (with_weights) ring.put_weights(w, ok, left, a.w_down);
+            // past I the row is padded with zeros to act_ld
+            if (with_acts) ring.put_acts(x, x_ok, static_cast<int>(a.act_ld - a.I) + left, lane, plane);
+        }
         R::step(ring.put, ring.base);
 #pragma unroll
         for (unsigned i = 0; i < 2 * MT; ++i) w[i / 2][i % 2] += parts * R::BLOCK;
-        if (x[0]) x[0] += parts * R::BLOCK;
+#pragma unroll
+        for (unsigned t = 0; t < NT; ++t) x[t] += parts * R::BLOCK;
         left -= static_cast<int>(parts * R::BLOCK);
         --put_left;
     };
@@ -638,29 +703,30 @@ moe_down(MoeDecodeArgs a) {
     for (unsigned u = warp; u < units; u += kWarps) {
         const unsigned g = sm.plan.group[u >> shift], n = group_count(g);
         const unsigned count = blocks_of(u);
-        float acc[1][MT][4], part[1][MT][4];
+        float acc[NT][MT][4], part[NT][MT][4];
         clear(acc);
         clear(part);
         for (unsigned b = 0; b < count; ++b) {
             put_step(true, true);
             cp_async_commit();
             cp_async_wait<R::STAGES - 1>();
-            ring.multiply(1, part, lane);
+            ring.multiply((n + 7) / 8, part, lane);
             R::step(ring.get, ring.base);
             if (b % kChain == kChain - 1) flush(acc, part);
         }
         flush(acc, part);
 #pragma unroll
-        for (unsigned e = 0; e < 2; ++e)
-            if (2 * c + e < n) {
-                float* sums = sm.sums[(u & (parts - 1)) * 2 * a.T +
-                                      sm.plan.lists[group_expert(g)][group_first(g) + 2 * c + e]];
+        for (unsigned t = 0; t < 2 * NT; ++t) {
+            const unsigned at = t / 2 * 8 + 2 * c + t % 2;
+            if (at < n) {
+                float* sums = sm.sums[(u & (parts - 1)) * 2 * a.T + sm.plan.lists[group_expert(g)][group_first(g) + at]];
 #pragma unroll
                 for (unsigned m = 0; m < MT; ++m) {
-                    sums[m * 16 + r] = acc[0][m][e];
-                    sums[m * 16 + r + 8] = acc[0][m][2 + e];
+                    sums[m * 16 + r] = acc[t / 2][m][t % 2];
+                    sums[m * 16 + r + 8] = acc[t / 2][m][2 + t % 2];
                 }
             }
+        }
     }
     __syncthreads();
     for (unsigned i = threadIdx.x; i < a.T * 16 * MT; i += kWarps * 32) {
@@ -690,10 +756,10 @@ cudaError_t launch_up(const MoeDecodeArgs& a, cudaStream_t s) {
     return launch_pdl(kernel, std::min(groups * tiles, static_cast<unsigned>(sm_count())), kWarps * 32, smem, s, a, tiles);
 }
 
-template <typename X, typename W, unsigned MT, bool VEC>
+template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 cudaError_t launch_down(const MoeDecodeArgs& a, cudaStream_t s) {
-    const auto kernel = moe_down<X, W, MT, VEC>;
-    const std::size_t smem = sizeof(typename Down<W, MT, VEC>::Smem);
+    const auto kernel = moe_down<X, W, MT, NT, VEC>;
+    const std::size_t smem = sizeof(typename Down<W, MT, NT, VEC>::Smem);
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, (a.H + 16 * MT - 1) / (16 * MT), kWarps * 32, smem, s, a);
@@ -712,8 +778,8 @@ cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     // 32 output rows per CTA as long as that reaches most SMs: the activations are read once for both tiles
     const bool tall = a.H >= 2368;
-    if (vec) return tall ? launch_down<X, W, 2, true>(a, s) : launch_down<X, W, 1, true>(a, s);
-    return tall ? launch_down<X, W, 2, false>(a, s) : launch_down<X, W, 1, false>(a, s);
+    if (vec) return tall ? launch_down<X, W, 2, 1, true>(a, s) : launch_down<X, W, 1, 1, true>(a, s);
+    return launch_down<X, W, 1, 2, false>(a, s);
 }
 
 }  // namespace
