@@ -1223,14 +1223,14 @@ __device__ __forceinline__ void run_part(const AttnKv4Args& a, const Part& p, Sm
 template <unsigned D>
 __device__ __forceinline__ unsigned fit_pairs(unsigned pairs, unsigned heads, unsigned share, Smem<D>& sm) {
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const unsigned most = share + warp * 2;
+    const unsigned most = share + warp * 4;
     unsigned ctas = 0;
     for (unsigned p = lane; p < pairs; p += 32) ctas += (sm.pair_units[p] + most - 1) / most;
     ctas = __reduce_add_sync(0xffffffffu, ctas) * heads;
     if (lane == 0) sm.fits[warp] = ctas <= gridDim.x;
     __syncthreads();
     for (unsigned w = 0; w < kWarps; ++w)
-        if (sm.fits[w]) return share + w * 2;
+        if (sm.fits[w]) return share + w * 4;
     return 0;
 }
 
@@ -1269,7 +1269,7 @@ attention_kv4_shares(AttnKv4Args a) {
     const unsigned share = max((work + gridDim.x - 1) / gridDim.x, min((all_units + pairs - 1) / pairs, kWarps));
 
     // ---- pairs on CTAs of their own, if that leaves no CTA with much more
-    // than its share: a second part costs a CTA what some 16 units do ----
+    // than its share: a second part costs a CTA what some 28 units do ----
     Part part;
     unsigned at = 0, stop = 0;    // else: the CTA's share of the list
     unsigned pair_begin = 0;      // units of earlier pairs, one head
