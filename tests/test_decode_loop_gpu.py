@@ -106,3 +106,31 @@ def test_attention_over_many_sequences(cuda, seqs, q_heads, kv_heads, queries, l
             # for a value next to zero, whose code and minimum cancel
             assert bool(((out[row].double() - want).abs() <= 2.0 ** -14 * (mag + 0.1)).all()), (s, i)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(4, 1, 128), (8, 1, 64)])
+def test_long_context_relative_to_its_output(cuda, q_heads, kv_heads, dim):
+    """Flat weights over many keys: outputs are a hundredth of a value, and
+    every sum that is larger and cancels shows."""
+    import torch
+
+    from aps2026_b200 import decode
+
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    n, page = 30001, 64
+    width = -(-n // page)
+    table = torch.randperm(width, generator=g, device="cuda").to(torch.int32).view(1, width)
+    cache = decode.KVCache4(width, page, kv_heads, dim, "cuda")
+    k, v = (torch.randn((n, kv_heads, dim), generator=g, device="cuda") for _ in range(2))
+    seq, pos = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    decode.kv4_append_gpu(k, v, seq, pos, cache, table)
+    decode.kv4_read_gpu(cache, table, seq, pos, k, v)
+    q = torch.randn((1, q_heads, dim), generator=g, device="cuda")
+    out = torch.empty_like(q)
+    decode.attention_kv4_gpu(q, cache, table, _i32([n]), out)
+    w = torch.softmax(q.double().view(kv_heads, -1, dim) @ k.double().permute(1, 2, 0) / math.sqrt(dim), -1)
+    want = (w @ v.double().transpose(0, 1)).view(1, q_heads, dim)
+    # each weight is off by some 2^-21 of itself (exp2, its argument) and p s
+    # by 2^-22, apart from each other, as the values are: the sum's error is
+    # that fraction of the sum. Three times it.
+    assert float((out.double() - want).norm() / want.norm()) < 3 * (2.0 ** -21)
