@@ -92,18 +92,18 @@ __device__ __forceinline__ unsigned scan_best(float score, unsigned lane, unsign
 // A lane per expert, 32 / SUB tokens per warp at a time: the code stays short
 // (it runs once per CTA, from a cold instruction cache).
 template <unsigned SUB>
-__device__ __forceinline__ void pick_experts(const MoeDecodeArgs& a, Plan& p) {
+__device__ __forceinline__ void pick_experts(const MoeDecodeArgs& a, unsigned from, unsigned tokens, Plan& p) {
     constexpr unsigned AT_ONCE = 32 / SUB, BATCH = 4;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, e = lane % SUB;
-    for (unsigned t0 = warp * AT_ONCE; t0 < a.T; t0 += kWarps * AT_ONCE * BATCH) {
+    for (unsigned t0 = warp * AT_ONCE; t0 < tokens; t0 += kWarps * AT_ONCE * BATCH) {
         float raw[BATCH];
 #pragma unroll
         for (unsigned i = 0; i < BATCH; ++i) {
             const unsigned t = t0 + i * kWarps * AT_ONCE + lane / SUB;
-            raw[i] = t < a.T && e < a.E ? __ldg(a.logits + static_cast<std::size_t>(t) * a.E + e) : 0.0f;
+            raw[i] = t < tokens && e < a.E ? __ldg(a.logits + static_cast<std::size_t>(from + t) * a.E + e) : 0.0f;
         }
 #pragma unroll 1
-        for (unsigned i = 0; i < BATCH && t0 + i * kWarps * AT_ONCE < a.T; ++i) {
+        for (unsigned i = 0; i < BATCH && t0 + i * kWarps * AT_ONCE < tokens; ++i) {
             const unsigned t = t0 + i * kWarps * AT_ONCE + lane / SUB;
             const float x = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
             const float score = quantize(x, a.quantum);
@@ -114,7 +114,7 @@ __device__ __forceinline__ void pick_experts(const MoeDecodeArgs& a, Plan& p) {
             const unsigned lo = min(first, second), hi = max(first, second);
             const float x0 = __shfl_sync(0xffffffffu, x, lane / SUB * SUB + lo);
             const float x1 = __shfl_sync(0xffffffffu, x, lane / SUB * SUB + hi);
-            if (e == 0 && t < a.T) {
+            if (e == 0 && t < tokens) {
                 float g0 = 0.5f, g1 = 0.5f;
                 if (a.gates == B2_GATES_SOFTMAX) {
                     const float m = fmaxf(x0, x1), p0 = expf(x0 - m), p1 = expf(x1 - m);
@@ -131,17 +131,17 @@ __device__ __forceinline__ void pick_experts(const MoeDecodeArgs& a, Plan& p) {
     }
 }
 
-// Routes the tokens and cuts every expert's into groups of CHUNK. Ends with a
-// barrier.
+// Routes tokens from .. from + tokens - 1 (counted from 0 in the plan) and cuts
+// every expert's into groups of CHUNK. Ends with a barrier.
 template <unsigned CHUNK>
-__device__ __forceinline__ void make_plan(const MoeDecodeArgs& a, Plan& p) {
+__device__ __forceinline__ void make_plan(const MoeDecodeArgs& a, unsigned from, unsigned tokens, Plan& p) {
     const unsigned t = threadIdx.x, lane = t & 31, warp = t / 32;
     if (warp < kMaxDecodeTokens / 32) p.mask[warp][lane] = 0;
     __syncthreads();
-    if (a.E <= 16) pick_experts<16>(a, p);
-    else pick_experts<32>(a, p);
+    if (a.E <= 16) pick_experts<16>(a, from, tokens, p);
+    else pick_experts<32>(a, from, tokens, p);
     __syncthreads();
-    if (t < 2 * a.T) {  // assignment t
+    if (t < 2 * tokens) {  // assignment t
         const unsigned token = t / 2, e = t % 2 ? p.pair[token] >> 8 : p.pair[token] & 0xFFu;
         unsigned rank = __popc(p.mask[token / 32][e] & ((1u << (token & 31)) - 1u));
         for (unsigned w = 0; w < token / 32; ++w) rank += __popc(p.mask[w][e]);
@@ -244,17 +244,96 @@ __device__ __forceinline__ void split_tf32(unsigned w, unsigned& hi, unsigned& l
     lo = __float_as_uint(__uint_as_float(w) - __uint_as_float(hi));
 }
 
+// Where a row that starts at any element lies in a stage: the 16-byte chunks
+// of memory that its block touches, side by side. They are brought by the four
+// lanes of the row and read across them from byte `skip` on.
+struct Span {
+    const unsigned char *from, *to;  // the tensor: nothing is read outside
+};
+template <typename T>
+__device__ __forceinline__ unsigned skip_of(const T* row) {
+    return static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(row)) & 15u;
+}
+__device__ __forceinline__ const unsigned char* chunk_of(const void* p) {
+    return reinterpret_cast<const unsigned char*>(reinterpret_cast<std::uintptr_t>(p) & ~std::uintptr_t(15));
+}
+// Whether all chunks of a row's `blocks` blocks of BYTES bytes are inside the tensor.
+template <unsigned BYTES>
+__device__ __forceinline__ bool is_inside(const void* row, unsigned blocks, const Span& span) {
+    const unsigned char* first = chunk_of(row);
+    return first >= span.from && first + (static_cast<std::size_t>(blocks) * BYTES + 16) <= span.to;
+}
+// Lane c's share of the BYTES bytes from `block` on and of the chunks around
+// them. inside: the tensor holds all of them.
+template <typename T, unsigned BYTES>
+__device__ __forceinline__ void copy_chunks(unsigned char* dst, const T* block, unsigned c, const Span& span, bool inside) {
+    const unsigned char* first = chunk_of(block);
+    if (inside) {
+        const unsigned to = smem_addr(dst) + c * 16;
+#pragma unroll
+        for (unsigned i = 0; i < BYTES / 16 + 1; i += 4)
+            if (i + 4 <= BYTES / 16 + 1 || i + c <= BYTES / 16)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + i * 16), "l"(first + c * 16 + i * 16)
+                             : "memory");
+        return;
+    }
+#pragma unroll 1
+    for (unsigned i = 0; i < BYTES / 16 + 1; i += 4) {
+        const unsigned j = i + c;
+        if (j > BYTES / 16) continue;
+        const unsigned char* chunk = first + j * 16;
+        if (chunk >= span.from) {
+            const std::ptrdiff_t there = span.to - chunk;
+            const int bytes = there >= 16 ? 16 : there > 0 ? static_cast<int>(there) : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + j * 16)),
+                         "l"(bytes ? chunk : first), "r"(bytes)
+                         : "memory");
+        } else {  // a tensor that starts inside a chunk
+            for (unsigned e = 0; e < 16; e += sizeof(T))
+                *reinterpret_cast<T*>(dst + j * 16 + e) =
+                    chunk + e >= span.from && chunk + e < span.to ? *reinterpret_cast<const T*>(chunk + e) : T(0.0f);
+        }
+    }
+}
+// Lane c's WORDS words of a row in a stage; elements from `left` on are zeros.
+template <typename T, unsigned WORDS>
+__device__ __forceinline__ void read_skewed(unsigned row, unsigned skip, unsigned c, int left, unsigned (&v)[WORDS]) {
+    const unsigned at = row + (skip & 12u) + c * WORDS * 4;
+    unsigned w[WORDS + 1];
+#pragma unroll
+    for (unsigned i = 0; i < WORDS + (sizeof(T) == 2); ++i)
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + i * 4));
+#pragma unroll
+    for (unsigned i = 0; i < WORDS; ++i) v[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (skip & 2u) * 8) : w[i];
+    constexpr int PER_WORD = 4 / sizeof(T);
+    if (left < static_cast<int>(WORDS) * PER_WORD)
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(WORDS); ++i)
+            if (left <= i * PER_WORD) v[i] = 0;
+            else if (PER_WORD == 2 && left == i * PER_WORD + 1) v[i] &= 0xFFFFu;
+}
+// What reading needs to know of the rows that it reads.
+template <unsigned MT, unsigned NT>
+struct Skew {
+    unsigned w[MT][2], x[NT];
+    int left;  // elements from the lane's k to the rows' ends
+};
+
 // The stages of one warp: MT 16-row tiles of a weight block (lane's rows r and
-// r + 8 of each) and NT 8-token tiles of activations (lane's token r), each
-// lane's bytes at its own place. VEC: every 16 bytes of a row of weights (XVEC:
-// the activations that meet them) are aligned, and inside the row or past it.
+// r + 8 of each) and NT 8-token tiles of activations (lane's token r). VEC:
+// every 16 bytes of a row of weights (XVEC: the activations that meet them)
+// are aligned, and inside the row or past it; then each lane's bytes have
+// their own place, and only the lane itself touches them. Else rows lie as
+// copy_chunks puts them.
 template <typename A, typename W, unsigned MT, unsigned NT, bool VEC, bool XVEC>
 struct Ring {
     using X = typename ActOf<A, W>::type;
     static constexpr unsigned PLANES = ActOf<A, W>::planes;
     static constexpr unsigned PER = kPer<W>, BLOCK = kBlock<W>;
     static constexpr unsigned XB = PLANES ? PLANES * 16 : PER * sizeof(X);  // bytes of a token per lane
-    static constexpr unsigned WEIGHTS = MT * 2 * 512, STAGE = WEIGHTS + NT * 32 * XB;
+    static constexpr unsigned WROW = 80, XROW = BLOCK * sizeof(X) + 16;     // bytes of an unaligned row
+    static constexpr unsigned WEIGHTS = MT * 2 * (VEC ? 512 : 8 * WROW), XTILE = XVEC ? 32 * XB : 8 * XROW;
+    static constexpr unsigned STAGE = WEIGHTS + NT * XTILE;
     static constexpr unsigned STAGES = kRing / STAGE < 6 ? kRing / STAGE : 6;
     static_assert(STAGES >= 2, "a ring of one stage");
     unsigned char* raw;       // the lane's place in the warp's first stage
@@ -267,6 +346,11 @@ struct Ring {
     static __device__ __forceinline__ void step(unsigned& at, unsigned base) {
         at += STAGE;
         if (at == base + STAGES * STAGE) at = base;
+    }
+    // Rows that lanes share: every lane has read the stage that is filled next
+    // (before put), every lane's copies are there (before multiply).
+    static __device__ __forceinline__ void meet() {
+        if (!VEC || !XVEC) __syncwarp();
     }
 
     // A stage that is inside its rows for all lanes. Rows and tokens that are
@@ -283,7 +367,7 @@ struct Ring {
 #pragma unroll
             for (unsigned n = 0; n < NT; ++n)
                 if ((x_ok >> n) & 1u) {
-                    const unsigned at = put + WEIGHTS + n * 32 * XB;
+                    const unsigned at = put + WEIGHTS + n * XTILE;
                     if constexpr (PLANES > 0) {
 #pragma unroll
                         for (unsigned q = 0; q < PLANES; ++q) copy_async16(at + q * 512, x[n] + q * plane);
@@ -299,7 +383,8 @@ struct Ring {
     }
     // w[m][i]: the lane's weights (row's start + k); ok: bit 2m + i set where
     // the row is there; left: weights from k to the row's end, if positive.
-    __device__ __forceinline__ void put_weights(const W* const (&w)[MT][2], unsigned ok, int left, const void* any) {
+    __device__ __forceinline__ void put_weights(const W* const (&w)[MT][2], unsigned ok, int left, const Span& span,
+                                                bool inside, unsigned lane) {
 #pragma unroll
         for (unsigned m = 0; m < MT; ++m)
 #pragma unroll
@@ -307,40 +392,22 @@ struct Ring {
                 const bool row = (ok >> (2 * m + i)) & 1u;
                 if (VEC) {
                     const bool have = row && left > 0;
-                    copy_async<16>(put + (m * 2 + i) * 512, have ? w[m][i] : any, have);
-                } else {
-                    unsigned char* dst = raw + (put - base) + (m * 2 + i) * 512;
-                    if (sizeof(W) == 2 && row && left > static_cast<int>(PER) && w[m][i] != any) {
-                        // 8 bf16 from the 4 (5, when they straddle) words that hold them: the
-                        // row goes on behind them, and the tensor began before them
-                        const std::uintptr_t at = reinterpret_cast<std::uintptr_t>(w[m][i]);
-                        const unsigned* words = reinterpret_cast<const unsigned*>(at & ~std::uintptr_t(3));
-                        const unsigned shift = (at & 2u) * 8;
-                        unsigned v[5];
-#pragma unroll
-                        for (unsigned e = 0; e < 4; ++e) v[e] = __ldg(words + e);
-                        v[4] = shift ? __ldg(words + 4) : 0u;
-                        *reinterpret_cast<uint4*>(dst) =
-                            make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
-                                       __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
-                        continue;
-                    }
-                    W v[PER];
-#pragma unroll
-                    for (unsigned e = 0; e < PER; ++e) v[e] = row && static_cast<int>(e) < left ? w[m][i][e] : W(0.0f);
-#pragma unroll
-                    for (unsigned e = 0; e < PER; ++e) reinterpret_cast<W*>(dst)[e] = v[e];
+                    copy_async<16>(put + (m * 2 + i) * 512, have ? static_cast<const void*>(w[m][i]) : span.from, have);
+                } else if (row) {
+                    const unsigned c = lane % 4;
+                    copy_chunks<W, 64>(raw + (put - base) - lane * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW,
+                                       w[m][i] - c * PER, c, span, inside);
                 }
             }
     }
     // x[n]: the lane's activations of token tile n (of the first plane); x_ok:
     // bit n set where there is a token.
     __device__ __forceinline__ void put_acts(const X* const (&x)[NT], unsigned x_ok, int left, unsigned lane,
-                                             std::size_t plane) {
+                                             std::size_t plane, const Span& span, bool inside) {
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
             if (!((x_ok >> n) & 1u)) continue;
-            const unsigned at = put + WEIGHTS + n * 32 * XB;
+            const unsigned at = put + WEIGHTS + n * XTILE;
             if (XVEC) {
                 const bool have = left > 0;  // x[n] is not read where there is none
                 if constexpr (PLANES > 0) {
@@ -355,40 +422,61 @@ struct Ring {
                     copy_async<8>(at - lane * 8, x[n], have);
                 }
             } else {
-                constexpr unsigned PIECE = XB >= 16 ? 16 / sizeof(X) : PER;  // elements per place
-                X v[PER];
-#pragma unroll
-                for (unsigned e = 0; e < PER; ++e) v[e] = static_cast<int>(e) < left ? x[n][e] : X(0.0f);
-                unsigned char* dst = raw + (at - base) - (XB == 8 ? lane * 8 : 0);
-#pragma unroll
-                for (unsigned e = 0; e < PER; ++e) reinterpret_cast<X*>(dst + e / PIECE * 512)[e % PIECE] = v[e];
+                const unsigned c = lane % 4;
+                copy_chunks<X, BLOCK * sizeof(X)>(raw + (at - base) - lane * 16 + lane / 4 * XROW, x[n] - c * PER, c, span, inside);
             }
         }
     }
 
     // part[n] += the stage's products for nt token tiles.
-    __device__ __forceinline__ void multiply(unsigned nt, float (&part)[NT][MT][4], unsigned lane) {
+    __device__ __forceinline__ void multiply(unsigned nt, float (&part)[NT][MT][4], unsigned lane,
+                                             const Skew<MT, NT>& skew) {
         constexpr unsigned PARTS = PLANES ? PLANES : kParts<X, W>;
         uint4 w[MT][2];
 #pragma unroll
         for (unsigned m = 0; m < MT; ++m) {
-            w[m][0] = lds16(get + m * 1024);
-            w[m][1] = lds16(get + m * 1024 + 512);
+            if constexpr (VEC) {
+                w[m][0] = lds16(get + m * 1024);
+                w[m][1] = lds16(get + m * 1024 + 512);
+            } else {
+#pragma unroll
+                for (unsigned i = 0; i < 2; ++i) {
+                    unsigned v[4];
+                    read_skewed<W>(get - lane * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW, skew.w[m][i], lane % 4, skew.left, v);
+                    w[m][i] = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
         }
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
             if (n >= nt) break;
-            const unsigned at = get + WEIGHTS + n * 32 * XB;
+            const unsigned at = get + WEIGHTS + n * XTILE;
+            unsigned v[PLANES ? 1 : XB / 4];  // raw activations
+            if constexpr (PLANES == 0) {
+                if constexpr (!XVEC) {
+                    read_skewed<X>(at - lane * 16 + lane / 4 * XROW, skew.x[n], lane % 4, skew.left, v);
+                } else if constexpr (XB == 8) {
+                    const uint2 y = lds8(at - lane * 8);
+                    v[0] = y.x; v[1] = y.y;
+                } else {
+#pragma unroll
+                    for (unsigned i = 0; i < XB / 16; ++i) {
+                        const uint4 y = lds16(at + i * 512);
+                        v[4 * i] = y.x; v[4 * i + 1] = y.y; v[4 * i + 2] = y.z; v[4 * i + 3] = y.w;
+                    }
+                }
+            }
             unsigned b[PARTS][4];
-            if constexpr (PLANES > 0 || (sizeof(X) == 2 && sizeof(W) == 2)) {  // in parts as it lies
+            if constexpr (PLANES > 0) {  // in parts as it lies
 #pragma unroll
                 for (unsigned q = 0; q < PARTS; ++q) {
-                    const uint4 v = lds16(at + q * 512);
-                    b[q][0] = v.x; b[q][1] = v.y; b[q][2] = v.z; b[q][3] = v.w;
+                    const uint4 y = lds16(at + q * 512);
+                    b[q][0] = y.x; b[q][1] = y.y; b[q][2] = y.z; b[q][3] = y.w;
                 }
+            } else if constexpr (sizeof(X) == 2 && sizeof(W) == 2) {
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) b[0][i] = v[i];
             } else if constexpr (sizeof(W) == 2) {  // x = three bf16 parts
-                const uint4 lo = lds16(at), hi = lds16(at + 512);
-                const unsigned v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (unsigned i = 0; i < 4; ++i) {
                     unsigned long long rest = f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
@@ -402,15 +490,11 @@ struct Ring {
                     }
                 }
             } else if constexpr (sizeof(X) == 4) {  // x = TF32 hi + lo
-                const uint4 v = lds16(at);
-                split_tf32(v.x, b[0][0], b[PARTS - 1][0]);
-                split_tf32(v.y, b[0][1], b[PARTS - 1][1]);
-                split_tf32(v.z, b[0][2], b[PARTS - 1][2]);
-                split_tf32(v.w, b[0][3], b[PARTS - 1][3]);
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) split_tf32(v[i], b[0][i], b[PARTS - 1][i]);
             } else {
-                const uint2 v = lds8(at - lane * 8);
-                b[0][0] = v.x << 16; b[0][1] = v.x & 0xFFFF0000u;
-                b[0][2] = v.y << 16; b[0][3] = v.y & 0xFFFF0000u;
+                b[0][0] = v[0] << 16; b[0][1] = v[0] & 0xFFFF0000u;
+                b[0][2] = v[1] << 16; b[0][3] = v[1] & 0xFFFF0000u;
             }
             if constexpr (sizeof(W) == 2) {
 #pragma unroll
@@ -490,53 +574,65 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     typename U::Smem& sm = *reinterpret_cast<typename U::Smem*>(smem_raw);
     pdl_begin();
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
-    make_plan<U::CHUNK>(a, sm.plan);
-    // equally many items per CTA, on as many CTAs as that takes
-    const unsigned items = sm.plan.groups * tiles;
-    const unsigned rounds = (items + gridDim.x - 1) / gridDim.x;
-    const unsigned ctas = (items + rounds - 1) / rounds;
+    make_plan<U::CHUNK>(a, 0, a.T, sm.plan);
+    // A round of a CTA is 2^shift items, kWarps >> shift warps each: a warp
+    // gets 4 k blocks per item, if there are items enough (2 blocks each cost
+    // 4 us of 64 at H = 1001; 8 instead of 4 gained nothing). Equally many
+    // rounds per CTA, on as many CTAs as that takes.
+    const unsigned items = sm.plan.groups * tiles, blocks = (a.H + R::BLOCK - 1) / R::BLOCK;
+    unsigned shift = 0;
+    while (shift < 2 && blocks << shift <= 2 * kWarps && items >> shift >= 2 * gridDim.x) ++shift;
+    const unsigned sets = (items + (1u << shift) - 1) >> shift, rounds = (sets + gridDim.x - 1) / gridDim.x;
+    const unsigned ctas = (sets + rounds - 1) / rounds;
     if (blockIdx.x >= ctas) return;
-
-    const unsigned blocks = (a.H + R::BLOCK - 1) / R::BLOCK;
-    const unsigned count = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0u;  // per item
+    const unsigned team = kWarps >> shift, mine = warp / team, at = warp % team, step = team * R::BLOCK;
+    const unsigned count = blocks > at ? (blocks - at + team - 1) / team : 0u;  // of a warp, per item
     R ring;
     ring.init(sm.ring[warp], lane);
+    const auto bytes = [](const void* p) { return static_cast<const unsigned char*>(p); };
+    const Span w_span{bytes(a.w_gate_up), bytes(static_cast<const W*>(a.w_gate_up) + std::size_t(2) * a.E * a.I * a.H)};
+    const Span x_span{bytes(a.x), bytes(static_cast<const X*>(a.x) + (a.T - 1) * a.ld_x + a.H)};
     // the end that fills
-    unsigned put_item = blockIdx.x, put_left = 0, ok = 0, x_ok = 0;
+    unsigned put_set = blockIdx.x, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
+    bool w_inside = false, x_inside = false;
     const W* w[1][2] = {};
     const X* x[NT] = {};
     const auto put_step = [&]() {
         if (put_left == 0) {
-            if (put_item >= items || count == 0) return;
-            const unsigned g = sm.plan.group[put_item / tiles], i = put_item % tiles * 8 + r;
-            const unsigned e = group_expert(g), k = warp * R::BLOCK + c * R::PER;
+            const unsigned item = (put_set << shift) + mine;
+            if (item >= items || count == 0) return;
+            const unsigned g = sm.plan.group[item / tiles], i = item % tiles * 8 + r;
+            const unsigned e = group_expert(g), k = at * R::BLOCK + c * R::PER;
             ok = i < a.I ? 3u : 0u;
             w[0][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H + k;
             w[0][1] = w[0][0] + static_cast<std::size_t>(a.I) * a.H;
+            w_inside = !VEC && is_inside<64>(w[0][0] - k, blocks, w_span) && is_inside<64>(w[0][1] - k, blocks, w_span);
+            x_inside = !VEC;
             x_ok = 0;
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
                 if (t * 8 + r < group_count(g)) {
                     x_ok |= 1u << t;
                     x[t] = static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x + k;
+                    if (!VEC) x_inside &= is_inside<R::BLOCK * sizeof(X)>(x[t] - k, blocks, x_span);
                 }
             left = static_cast<int>(a.H) - static_cast<int>(k);
             put_left = count;
-            put_item += ctas;
+            put_set += ctas;
         }
         if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
             if constexpr (VEC) ring.put_whole(w, ok, true, x, x_ok, true, lane, 0);
         } else {
-            ring.put_weights(w, ok, left, a.w_gate_up);
-            ring.put_acts(x, x_ok, left, lane, 0);
+            ring.put_weights(w, ok, left, w_span, w_inside, lane);
+            ring.put_acts(x, x_ok, left, lane, 0, x_span, x_inside);
         }
         R::step(ring.put, ring.base);
-        w[0][0] += kWarps * R::BLOCK;
-        w[0][1] += kWarps * R::BLOCK;
+        w[0][0] += step;
+        w[0][1] += step;
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t) x[t] += kWarps * R::BLOCK;
-        left -= static_cast<int>(kWarps * R::BLOCK);
+        for (unsigned t = 0; t < NT; ++t) x[t] += step;
+        left -= static_cast<int>(step);
         --put_left;
     };
 #pragma unroll 1
@@ -545,35 +641,56 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
         cp_async_commit();
     }
     unsigned buffer = 0;
-    for (unsigned item = blockIdx.x; item < items; item += ctas, buffer ^= 1) {
-        const unsigned g = sm.plan.group[item / tiles], i0 = item % tiles * 8;
-        const unsigned e = group_expert(g), n = group_count(g), nt = (n + 7) / 8;
-        float acc[NT][1][4], part[NT][1][4];
-        clear(acc);
-        clear(part);
-        for (unsigned i = 0; i < count; ++i) {
-            put_step();
-            cp_async_commit();
-            cp_async_wait<R::STAGES - 1>();
-            ring.multiply(nt, part, lane);
-            R::step(ring.get, ring.base);
-            if (i % kChain == kChain - 1) flush(acc, part);
-        }
-        flush(acc, part);
+    for (unsigned set = blockIdx.x; set << shift < items; set += ctas, buffer ^= 1) {
         auto& sums = sm.sums[buffer];
+        const unsigned item = (set << shift) + mine;
+        if (item < items) {
+            const unsigned g = sm.plan.group[item / tiles], n = group_count(g), nt = (n + 7) / 8;
+            float acc[NT][1][4], part[NT][1][4];
+            clear(acc);
+            clear(part);
+            Skew<1, NT> skew{};
+            if constexpr (!VEC) {
+                const unsigned e = group_expert(g), i = item % tiles * 8 + r;
+                const W* row = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H;
+                skew.w[0][0] = skip_of(row);
+                skew.w[0][1] = skip_of(row + static_cast<std::size_t>(a.I) * a.H);
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t)
-            if (t < nt)
+                for (unsigned t = 0; t < NT; ++t)
+                    if (t * 8 + r < n)
+                        skew.x[t] = skip_of(static_cast<const X*>(a.x) + sm.plan.lists[e][group_first(g) + t * 8 + r] / 2 * a.ld_x);
+                skew.left = static_cast<int>(a.H) - static_cast<int>(at * R::BLOCK + c * R::PER);
+            }
+            for (unsigned i = 0; i < count; ++i) {
+                R::meet();
+                put_step();
+                cp_async_commit();
+                cp_async_wait<R::STAGES - 1>();
+                R::meet();
+                ring.multiply(nt, part, lane, skew);
+                skew.left -= static_cast<int>(step);
+                R::step(ring.get, ring.base);
+                if (i % kChain == kChain - 1) flush(acc, part);
+            }
+            flush(acc, part);
 #pragma unroll
-                for (unsigned i = 0; i < 4; ++i) sums[warp][r + i / 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][0][i];
+            for (unsigned t = 0; t < NT; ++t)
+                if (t < nt)
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i) sums[warp][r + i / 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][0][i];
+        }
         __syncthreads();  // also: everyone has read the other buffer
-        const unsigned row = threadIdx.x % 8, t = threadIdx.x / 8;
-        if (t < n && i0 + row < a.act_ld) {
+        const unsigned row = threadIdx.x % 8, t = threadIdx.x / 8 % U::CHUNK, which = threadIdx.x / (8 * U::CHUNK);
+        const unsigned done = (set << shift) + which, i0 = done % tiles * 8;
+        if (which >> shift || done >= items) continue;
+        const unsigned g = sm.plan.group[done / tiles], e = group_expert(g);
+        if (t < group_count(g) && i0 + row < a.act_ld) {
             float gate = 0.0f, up = 0.0f;
 #pragma unroll
             for (unsigned v = 0; v < kWarps; ++v) {
-                gate += sums[v][row][t];
-                up += sums[v][row + 8][t];
+                if (v >= team) break;
+                gate += sums[which * team + v][row][t];
+                up += sums[which * team + v][row + 8][t];
             }
             const unsigned to = sm.plan.lists[e][group_first(g) + t];
             const std::size_t at = static_cast<std::size_t>(to) * a.act_ld + i0 + row;
@@ -611,7 +728,7 @@ struct Down {
 
 template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, 1)
-moe_down(MoeDecodeArgs a) {
+moe_down(MoeDecodeArgs a, unsigned per) {
     using D = Down<W, MT, NT, VEC>;
     using R = typename D::R;
     using Act = typename R::X;
@@ -622,7 +739,8 @@ moe_down(MoeDecodeArgs a) {
     // launch start.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
-    make_plan<8 * NT>(a, sm.plan);
+    const unsigned t0 = blockIdx.y * per, T = min(per, a.T - t0);  // the CTA's tokens
+    make_plan<8 * NT>(a, t0, T, sm.plan);
     // k is cut in 2^shift parts so that the warps' loads even out: the fewest
     // rounds of (a part's blocks + 4, what a unit costs besides)
     const unsigned groups = sm.plan.groups, blocks = (a.I + R::BLOCK - 1) / R::BLOCK;
@@ -630,7 +748,7 @@ moe_down(MoeDecodeArgs a) {
 #pragma unroll
     for (unsigned s = 0; s < 4; ++s) {
         const unsigned cost = (((groups << s) + kWarps - 1) / kWarps) * (((blocks + (1u << s) - 1) >> s) + 4);
-        if (((2 * a.T) << s) <= kDownPartials && (1u << s) <= blocks && cost < best) {
+        if (((2 * T) << s) <= kDownPartials && (1u << s) <= blocks && cost < best) {
             best = cost;
             shift = s;
         }
@@ -640,11 +758,14 @@ moe_down(MoeDecodeArgs a) {
     const std::size_t plane = static_cast<std::size_t>(2) * a.T * a.act_ld;
     R ring;
     ring.init(sm.ring[warp], lane);
+    const Span w_span{static_cast<const unsigned char*>(a.w_down),
+                      reinterpret_cast<const unsigned char*>(static_cast<const W*>(a.w_down) + std::size_t(a.E) * a.H * a.I)};
 
     // The warp's blocks are those of its units u = warp, warp + kWarps, ...,
     // one after the other through the ring.
     unsigned put_u = warp, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
+    bool inside = false;
     const W* w[MT][2] = {};
     const Act* x[NT] = {};
     const auto put_step = [&](bool with_weights, bool with_acts) {
@@ -653,11 +774,13 @@ moe_down(MoeDecodeArgs a) {
             const unsigned g = sm.plan.group[put_u >> shift], e = group_expert(g);
             const unsigned k = (put_u & (parts - 1)) * R::BLOCK + c * R::PER;
             ok = 0;
+            inside = !VEC;
 #pragma unroll
             for (unsigned i = 0; i < 2 * MT; ++i) {
                 const unsigned h = h0 + r + 8 * i;
                 w[i / 2][i % 2] = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I + k;
                 if (h < a.H) ok |= 1u << i;
+                if (!VEC && h < a.H) inside &= is_inside<64>(w[i / 2][i % 2] - k, blocks, w_span);
             }
             x_ok = 0;
 #pragma unroll
@@ -665,7 +788,7 @@ moe_down(MoeDecodeArgs a) {
                 if (t * 8 + r < group_count(g)) {
                     x_ok |= 1u << t;
                     x[t] = static_cast<const Act*>(a.act) +
-                           static_cast<std::size_t>(sm.plan.lists[e][group_first(g) + t * 8 + r]) * a.act_ld + k;
+                           static_cast<std::size_t>(2 * t0 + sm.plan.lists[e][group_first(g) + t * 8 + r]) * a.act_ld + k;
                 }
             left = static_cast<int>(a.I) - static_cast<int>(k);
             put_left = blocks_of(put_u);
@@ -674,9 +797,9 @@ moe_down(MoeDecodeArgs a) {
         if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
             if constexpr (VEC) ring.put_whole(w, ok, with_weights, x, x_ok, with_acts, lane, plane);
         } else {
-            if (with_weights) ring.put_weights(w, ok, left, a.w_down);
+            if (with_weights) ring.put_weights(w, ok, left, w_span, inside, lane);
             // past I the row is padded with zeros to act_ld
-            if (with_acts) ring.put_acts(x, x_ok, static_cast<int>(a.act_ld - a.I) + left, lane, plane);
+            if (with_acts) ring.put_acts(x, x_ok, static_cast<int>(a.act_ld - a.I) + left, lane, plane, w_span, false);
         }
         R::step(ring.put, ring.base);
 #pragma unroll
@@ -706,11 +829,22 @@ moe_down(MoeDecodeArgs a) {
         float acc[NT][MT][4], part[NT][MT][4];
         clear(acc);
         clear(part);
+        Skew<MT, NT> skew{};
+        if constexpr (!VEC) {
+#pragma unroll
+            for (unsigned i = 0; i < 2 * MT; ++i)
+                skew.w[i / 2][i % 2] = skip_of(static_cast<const W*>(a.w_down) +
+                                               (static_cast<std::size_t>(group_expert(g)) * a.H + h0 + r + 8 * i) * a.I);
+            skew.left = static_cast<int>(a.I) - static_cast<int>((u & (parts - 1)) * R::BLOCK + c * R::PER);
+        }
         for (unsigned b = 0; b < count; ++b) {
+            R::meet();
             put_step(true, true);
             cp_async_commit();
             cp_async_wait<R::STAGES - 1>();
-            ring.multiply((n + 7) / 8, part, lane);
+            R::meet();
+            ring.multiply((n + 7) / 8, part, lane, skew);
+            skew.left -= static_cast<int>(parts * R::BLOCK);
             R::step(ring.get, ring.base);
             if (b % kChain == kChain - 1) flush(acc, part);
         }
@@ -719,7 +853,7 @@ moe_down(MoeDecodeArgs a) {
         for (unsigned t = 0; t < 2 * NT; ++t) {
             const unsigned at = t / 2 * 8 + 2 * c + t % 2;
             if (at < n) {
-                float* sums = sm.sums[(u & (parts - 1)) * 2 * a.T + sm.plan.lists[group_expert(g)][group_first(g) + at]];
+                float* sums = sm.sums[(u & (parts - 1)) * 2 * T + sm.plan.lists[group_expert(g)][group_first(g) + at]];
 #pragma unroll
                 for (unsigned m = 0; m < MT; ++m) {
                     sums[m * 16 + r] = acc[t / 2][m][t % 2];
@@ -729,16 +863,16 @@ moe_down(MoeDecodeArgs a) {
         }
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < a.T * 16 * MT; i += kWarps * 32) {
+    for (unsigned i = threadIdx.x; i < T * 16 * MT; i += kWarps * 32) {
         const unsigned t = i / (16 * MT), h = i % (16 * MT);
         if (h0 + h >= a.H) continue;
         float y[2] = {0.0f, 0.0f};
         for (unsigned p = 0; p < parts; ++p) {
-            y[0] += sm.sums[p * 2 * a.T + 2 * t][h];
-            y[1] += sm.sums[p * 2 * a.T + 2 * t + 1][h];
+            y[0] += sm.sums[p * 2 * T + 2 * t][h];
+            y[1] += sm.sums[p * 2 * T + 2 * t + 1][h];
         }
         const float v = sm.plan.gate[2 * t] * y[0] + sm.plan.gate[2 * t + 1] * y[1];
-        X* out = static_cast<X*>(a.out) + t * a.ld_out + h0 + h;
+        X* out = static_cast<X*>(a.out) + (t0 + t) * a.ld_out + h0 + h;
         if constexpr (sizeof(X) == 2) *out = __float2bfloat16_rn(v);
         else *out = v;
     }
@@ -762,7 +896,13 @@ cudaError_t launch_down(const MoeDecodeArgs& a, cudaStream_t s) {
     const std::size_t smem = sizeof(typename Down<W, MT, NT, VEC>::Smem);
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, (a.H + 16 * MT - 1) / (16 * MT), kWarps * 32, smem, s, a);
+    // as long as rows alone leave SMs without a CTA, the tokens are cut in two,
+    // down to 16 (128 tokens of H = 1001: 63 CTAs -> 126)
+    const unsigned rows = (a.H + 16 * MT - 1) / (16 * MT);
+    unsigned cuts = 1;
+    while (2 * cuts * rows <= static_cast<unsigned>(sm_count()) && a.T >= 32 * cuts) cuts *= 2;
+    const unsigned per = (a.T + cuts - 1) / cuts;
+    return launch_pdl(kernel, dim3(rows, (a.T + per - 1) / per), kWarps * 32, smem, s, a, per);
 }
 
 template <typename X, typename W>
@@ -772,14 +912,13 @@ cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
     // 16 tokens per group where the experts have more than 4 on average: fewer
     // experts are read twice; else 8, whose smaller stages leave more weights in flight
     const bool wide = 2 * a.T > 4 * a.E;
-    cudaError_t e = !vec   ? launch_up<X, W, 2, false>(a, s)
-                    : wide ? launch_up<X, W, 2, true>(a, s)
-                           : launch_up<X, W, 1, true>(a, s);
+    cudaError_t e = vec ? wide ? launch_up<X, W, 2, true>(a, s) : launch_up<X, W, 1, true>(a, s)
+                        : wide ? launch_up<X, W, 2, false>(a, s) : launch_up<X, W, 1, false>(a, s);
     if (e != cudaSuccess) return e;
     // 32 output rows per CTA as long as that reaches most SMs: the activations are read once for both tiles
     const bool tall = a.H >= 2368;
     if (vec) return tall ? launch_down<X, W, 2, 1, true>(a, s) : launch_down<X, W, 1, 1, true>(a, s);
-    return launch_down<X, W, 1, 2, false>(a, s);
+    return wide ? launch_down<X, W, 1, 2, false>(a, s) : launch_down<X, W, 1, 1, false>(a, s);
 }
 
 }  // namespace
