@@ -553,22 +553,23 @@ __device__ __forceinline__ void flush(float (&acc)[NT][MT][4], float (&part)[NT]
 
 // ---- launch 1 ---------------------------------------------------------------------------
 
-// Item j: group j / tiles, rows j % tiles * 8 ... of its gate and up.
-template <typename X, typename W, unsigned NT, bool VEC>
+// Item j: group j / tiles, rows j % tiles * 8 MT ... of its gate and up.
+template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 struct Up {
-    using R = Ring<X, W, 1, NT, VEC, VEC>;
-    static constexpr unsigned CHUNK = 8 * NT;
+    using R = Ring<X, W, MT, NT, VEC, VEC>;
+    static constexpr unsigned ROWS = 8 * MT, CHUNK = 8 * NT;
+    static constexpr unsigned BUFFERS = MT == 1 ? 2 : 1;
     struct Smem {
         alignas(16) unsigned char ring[kWarps][kRing];
-        float sums[2][kWarps][16][CHUNK + 1];  // of items j and j + 1
+        float sums[BUFFERS][kWarps][16 * MT][CHUNK + 1];
         Plan plan;
     };
 };
 
-template <typename X, typename W, unsigned NT, bool VEC>
+template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, 1)
 moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
-    using U = Up<X, W, NT, VEC>;
+    using U = Up<X, W, MT, NT, VEC>;
     using R = typename U::R;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     typename U::Smem& sm = *reinterpret_cast<typename U::Smem*>(smem_raw);
@@ -581,7 +582,7 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     // rounds per CTA, on as many CTAs as that takes.
     const unsigned items = sm.plan.groups * tiles, blocks = (a.H + R::BLOCK - 1) / R::BLOCK;
     unsigned shift = 0;
-    while (shift < 2 && blocks << shift <= 2 * kWarps && items >> shift >= 2 * gridDim.x) ++shift;
+    while (shift < (MT == 1 ? 2 : 1) && blocks << shift <= 2 * kWarps && items >> shift >= 2 * gridDim.x) ++shift;
     const unsigned sets = (items + (1u << shift) - 1) >> shift, rounds = (sets + gridDim.x - 1) / gridDim.x;
     const unsigned ctas = (sets + rounds - 1) / rounds;
     if (blockIdx.x >= ctas) return;
@@ -596,19 +597,24 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     unsigned put_set = blockIdx.x, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
     bool w_inside = false, x_inside = false;
-    const W* w[1][2] = {};
+    const W* w[MT][2] = {};
     const X* x[NT] = {};
     const auto put_step = [&]() {
         if (put_left == 0) {
             const unsigned item = (put_set << shift) + mine;
             if (item >= items || count == 0) return;
-            const unsigned g = sm.plan.group[item / tiles], i = item % tiles * 8 + r;
+            const unsigned g = sm.plan.group[item / tiles], i = item % tiles * U::ROWS + r;
             const unsigned e = group_expert(g), k = at * R::BLOCK + c * R::PER;
-            ok = i < a.I ? 3u : 0u;
-            w[0][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H + k;
-            w[0][1] = w[0][0] + static_cast<std::size_t>(a.I) * a.H;
-            w_inside = !VEC && is_inside<64>(w[0][0] - k, blocks, w_span) && is_inside<64>(w[0][1] - k, blocks, w_span);
-            x_inside = !VEC;
+            ok = 0;
+            w_inside = x_inside = !VEC;
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                w[m][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i + m * 8) * a.H + k;
+                w[m][1] = w[m][0] + static_cast<std::size_t>(a.I) * a.H;
+                if (i + m * 8 >= a.I) continue;
+                ok |= 3u << 2 * m;
+                if (!VEC) w_inside &= is_inside<64>(w[m][0] - k, blocks, w_span) && is_inside<64>(w[m][1] - k, blocks, w_span);
+            }
             x_ok = 0;
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
@@ -628,8 +634,8 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             ring.put_acts(x, x_ok, left, lane, 0, x_span, x_inside);
         }
         R::step(ring.put, ring.base);
-        w[0][0] += step;
-        w[0][1] += step;
+#pragma unroll
+        for (unsigned i = 0; i < 2 * MT; ++i) w[i / 2][i % 2] += step;
 #pragma unroll
         for (unsigned t = 0; t < NT; ++t) x[t] += step;
         left -= static_cast<int>(step);
@@ -641,20 +647,23 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
         cp_async_commit();
     }
     unsigned buffer = 0;
-    for (unsigned set = blockIdx.x; set << shift < items; set += ctas, buffer ^= 1) {
+    for (unsigned set = blockIdx.x; set << shift < items; set += ctas, buffer = U::BUFFERS - 1 - buffer) {
         auto& sums = sm.sums[buffer];
         const unsigned item = (set << shift) + mine;
         if (item < items) {
             const unsigned g = sm.plan.group[item / tiles], n = group_count(g), nt = (n + 7) / 8;
-            float acc[NT][1][4], part[NT][1][4];
+            float acc[NT][MT][4], part[NT][MT][4];
             clear(acc);
             clear(part);
-            Skew<1, NT> skew{};
+            Skew<MT, NT> skew{};
             if constexpr (!VEC) {
-                const unsigned e = group_expert(g), i = item % tiles * 8 + r;
+                const unsigned e = group_expert(g), i = item % tiles * U::ROWS + r;
                 const W* row = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i) * a.H;
-                skew.w[0][0] = skip_of(row);
-                skew.w[0][1] = skip_of(row + static_cast<std::size_t>(a.I) * a.H);
+#pragma unroll
+                for (unsigned m = 0; m < MT; ++m) {
+                    skew.w[m][0] = skip_of(row + std::size_t(8 * m) * a.H);
+                    skew.w[m][1] = skip_of(row + (std::size_t(a.I) + 8 * m) * a.H);
+                }
 #pragma unroll
                 for (unsigned t = 0; t < NT; ++t)
                     if (t * 8 + r < n)
@@ -677,20 +686,20 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             for (unsigned t = 0; t < NT; ++t)
                 if (t < nt)
 #pragma unroll
-                    for (unsigned i = 0; i < 4; ++i) sums[warp][r + i / 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][0][i];
+                    for (unsigned i = 0; i < 4 * MT; ++i)
+                        sums[warp][i / 4 * 16 + r + i / 2 % 2 * 8][t * 8 + 2 * c + i % 2] = acc[t][i / 4][i % 4];
         }
         __syncthreads();  // also: everyone has read the other buffer
-        const unsigned row = threadIdx.x % 8, t = threadIdx.x / 8 % U::CHUNK, which = threadIdx.x / (8 * U::CHUNK);
-        const unsigned done = (set << shift) + which, i0 = done % tiles * 8;
-        if (which >> shift || done >= items) continue;
-        const unsigned g = sm.plan.group[done / tiles], e = group_expert(g);
-        if (t < group_count(g) && i0 + row < a.act_ld) {
+        const unsigned row = threadIdx.x % U::ROWS, t = threadIdx.x / U::ROWS % U::CHUNK;
+        const unsigned which = threadIdx.x / (U::ROWS * U::CHUNK), done = (set << shift) + which;
+        const unsigned i0 = done % tiles * U::ROWS, g = done < items ? sm.plan.group[done / tiles] : 0u, e = group_expert(g);
+        if (which >> shift == 0 && t < group_count(g) && i0 + row < a.act_ld) {
             float gate = 0.0f, up = 0.0f;
 #pragma unroll
             for (unsigned v = 0; v < kWarps; ++v) {
                 if (v >= team) break;
-                gate += sums[which * team + v][row][t];
-                up += sums[which * team + v][row + 8][t];
+                gate += sums[which * team + v][row / 8 * 16 + row % 8][t];
+                up += sums[which * team + v][row / 8 * 16 + row % 8 + 8][t];
             }
             const unsigned to = sm.plan.lists[e][group_first(g) + t];
             const std::size_t at = static_cast<std::size_t>(to) * a.act_ld + i0 + row;
@@ -711,6 +720,7 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                 static_cast<unsigned*>(a.act)[plane + at] = lo;
             }
         }
+        if (U::BUFFERS == 1) __syncthreads();
     }
 }
 
@@ -878,13 +888,14 @@ moe_down(MoeDecodeArgs a, unsigned per) {
     }
 }
 
-template <typename X, typename W, unsigned NT, bool VEC>
+template <typename X, typename W, unsigned MT, unsigned NT, bool VEC>
 cudaError_t launch_up(const MoeDecodeArgs& a, cudaStream_t s) {
-    const unsigned tiles = (a.I + 7) / 8, chunk = 8 * NT;
-    // an expert's last group may be partial, the others hold `chunk` assignments
-    const unsigned groups = std::min(2 * a.T, std::min(a.E, 2 * a.T) + 2 * a.T / chunk);
-    const auto kernel = moe_gate_up<X, W, NT, VEC>;
-    const std::size_t smem = sizeof(typename Up<X, W, NT, VEC>::Smem);
+    using U = Up<X, W, MT, NT, VEC>;
+    const unsigned tiles = (a.I + U::ROWS - 1) / U::ROWS;
+    // an expert's last group may be partial, the others hold CHUNK assignments
+    const unsigned groups = std::min(2 * a.T, std::min(a.E, 2 * a.T) + 2 * a.T / U::CHUNK);
+    const auto kernel = moe_gate_up<X, W, MT, NT, VEC>;
+    const std::size_t smem = sizeof(typename U::Smem);
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, std::min(groups * tiles, static_cast<unsigned>(sm_count())), kWarps * 32, smem, s, a, tiles);
@@ -912,8 +923,8 @@ cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
     // 16 tokens per group where the experts have more than 4 on average: fewer
     // experts are read twice; else 8, whose smaller stages leave more weights in flight
     const bool wide = 2 * a.T > 4 * a.E;
-    cudaError_t e = vec ? wide ? launch_up<X, W, 2, true>(a, s) : launch_up<X, W, 1, true>(a, s)
-                        : wide ? launch_up<X, W, 2, false>(a, s) : launch_up<X, W, 1, false>(a, s);
+    cudaError_t e = vec ? wide ? launch_up<X, W, 2, 2, true>(a, s) : launch_up<X, W, 1, 1, true>(a, s)
+                        : wide ? launch_up<X, W, 2, 2, false>(a, s) : launch_up<X, W, 1, 1, false>(a, s);
     if (e != cudaSuccess) return e;
     // 32 output rows per CTA as long as that reaches most SMs: the activations are read once for both tiles
     const bool tall = a.H >= 2368;
