@@ -4,7 +4,8 @@ Each CUDA translation unit is compiled by nvcc (``-gencode
 arch=compute_100a,code=sm_100a -lineinfo -O3``, IEEE division and square
 root, no fast-math: the routing quantiser and the LayerNorm need them), the
 host C++ by g++, and everything is linked into one shared library next to
-this file. Objects go to ``aps2026_b200/_build`` and are rebuilt only when a
+this file; pyext/ becomes _decode_calls.so, the Python calls of the decode step
+(g++ against torch's headers, linked to the library). Objects go to ``aps2026_b200/_build`` and are rebuilt only when a
 source or header is newer.
 
 Run as ``python -m aps2026_b200.build [-v]`` (``-v`` prints ptxas register /
@@ -23,6 +24,8 @@ CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libaps2026_b200.so"
 INCLUDE = HERE.parent / "include"
+PYEXT = HERE / "pyext" / "decode_calls.cpp"
+PYEXT_LIB = HERE / "_decode_calls.so"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CXX = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else "g++"
@@ -59,6 +62,25 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_pyext() -> None:
+    newest = max([PYEXT.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
+    if PYEXT_LIB.exists() and PYEXT_LIB.stat().st_mtime >= newest:
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths(), str(Path(NVCC).parents[1] / "include"), sysconfig.get_paths()["include"]]
+    libs = cpp_extension.library_paths()[0]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(x for i in includes for x in ("-isystem", i)), str(PYEXT), "-o", str(PYEXT_LIB), f"-L{libs}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{libs}", f"-L{HERE}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+
+
 def build(verbose: bool = False) -> Path:
     """Compiles every source (in parallel) and links the shared library."""
     BUILD.mkdir(exist_ok=True)
@@ -71,6 +93,7 @@ def build(verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    _build_pyext()
     return LIB
 
 
