@@ -576,15 +576,23 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     pdl_begin();
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
     make_plan<U::CHUNK>(a, 0, a.T, sm.plan);
-    // A round of a CTA is 2^shift items, kWarps >> shift warps each: a warp
-    // gets 4 k blocks per item, if there are items enough (2 blocks each cost
-    // 4 us of 64 at H = 1001; 8 instead of 4 gained nothing). Equally many
-    // rounds per CTA, on as many CTAs as that takes.
+    // A round of a CTA is 2^shift items, kWarps >> shift warps each. With few k
+    // blocks a warp has little to do between two rounds' ends, which cost it
+    // what 2 blocks do; then fewer warps per item are better, if that fits the
+    // number of items (H = 256: 23 instead of 39 us; from 4 blocks per warp on,
+    // nothing is gained). Equally many rounds per CTA, on as many CTAs as that takes.
     const unsigned items = sm.plan.groups * tiles, blocks = (a.H + R::BLOCK - 1) / R::BLOCK;
-    unsigned shift = 0;
-    while (shift < (MT == 1 ? 2 : 1) && blocks << shift <= 2 * kWarps && items >> shift >= 2 * gridDim.x) ++shift;
-    const unsigned sets = (items + (1u << shift) - 1) >> shift, rounds = (sets + gridDim.x - 1) / gridDim.x;
-    const unsigned ctas = (sets + rounds - 1) / rounds;
+    unsigned shift = 0, ctas = 0;
+    for (unsigned s = 0, best = ~0u; s < (MT == 1 ? 3 : 2); ++s) {
+        if (s && blocks << s > 4 * kWarps) break;
+        const unsigned sets = (items + (1u << s) - 1) >> s, rounds = (sets + gridDim.x - 1) / gridDim.x;
+        const unsigned cost = rounds * ((((blocks << s) + kWarps - 1) / kWarps) + 2);
+        if (cost < best) {
+            best = cost;
+            shift = s;
+            ctas = (sets + rounds - 1) / rounds;
+        }
+    }
     if (blockIdx.x >= ctas) return;
     const unsigned team = kWarps >> shift, mine = warp / team, at = warp % team, step = team * R::BLOCK;
     const unsigned count = blocks > at ? (blocks - at + team - 1) / team : 0u;  // of a warp, per item
