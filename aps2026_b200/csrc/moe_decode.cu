@@ -263,37 +263,39 @@ __device__ __forceinline__ bool is_inside(const void* row, unsigned blocks, cons
     const unsigned char* first = chunk_of(row);
     return first >= span.from && first + (static_cast<std::size_t>(blocks) * BYTES + 16) <= span.to;
 }
-// Lane c's share of the BYTES bytes from `block` on and of the chunks around
-// them. inside: the tensor holds all of them.
+// Lane c's share of a block of BYTES bytes and of the chunks around them:
+// chunks c, c + 4, ... of the row's, the first of which is at `chunk` and goes
+// to `dst`. inside: the tensor holds all of them.
 template <typename T, unsigned BYTES>
-__device__ __forceinline__ void copy_chunks(unsigned char* dst, const T* block, unsigned c, const Span& span, bool inside) {
-    const unsigned char* first = chunk_of(block);
+__device__ __forceinline__ void copy_chunks(unsigned char* dst, const void* chunk, unsigned c, const Span& span, bool inside) {
+    const unsigned char* from = static_cast<const unsigned char*>(chunk);
     if (inside) {
-        const unsigned to = smem_addr(dst) + c * 16;
+        const unsigned to = smem_addr(dst);
 #pragma unroll
         for (unsigned i = 0; i < BYTES / 16 + 1; i += 4)
             if (i + 4 <= BYTES / 16 + 1 || i + c <= BYTES / 16)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + i * 16), "l"(first + c * 16 + i * 16)
-                             : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + i * 16), "l"(from + i * 16) : "memory");
         return;
     }
 #pragma unroll 1
-    for (unsigned i = 0; i < BYTES / 16 + 1; i += 4) {
-        const unsigned j = i + c;
-        if (j > BYTES / 16) continue;
-        const unsigned char* chunk = first + j * 16;
-        if (chunk >= span.from) {
-            const std::ptrdiff_t there = span.to - chunk;
+    for (unsigned i = 0; i + c <= BYTES / 16; i += 4, from += 64, dst += 64) {
+        if (from >= span.from) {
+            const std::ptrdiff_t there = span.to - from;
             const int bytes = there >= 16 ? 16 : there > 0 ? static_cast<int>(there) : 0;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + j * 16)),
-                         "l"(bytes ? chunk : first), "r"(bytes)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)),
+                         "l"(bytes ? from : chunk_of(span.from) + 16), "r"(bytes)
                          : "memory");
         } else {  // a tensor that starts inside a chunk
             for (unsigned e = 0; e < 16; e += sizeof(T))
-                *reinterpret_cast<T*>(dst + j * 16 + e) =
-                    chunk + e >= span.from && chunk + e < span.to ? *reinterpret_cast<const T*>(chunk + e) : T(0.0f);
+                *reinterpret_cast<T*>(dst + e) =
+                    from + e >= span.from && from + e < span.to ? *reinterpret_cast<const T*>(from + e) : T(0.0f);
         }
     }
+}
+// Where lane c's chunks of a row begin, at its block `at`.
+template <typename T>
+__device__ __forceinline__ const T* lane_chunk(const T* row, unsigned block_bytes, unsigned at, unsigned c) {
+    return reinterpret_cast<const T*>(chunk_of(row) + (static_cast<std::size_t>(at) * block_bytes + c * 16));
 }
 // Lane c's WORDS words of a row in a stage; elements from `left` on are zeros.
 template <typename T, unsigned WORDS>
@@ -394,9 +396,9 @@ struct Ring {
                     const bool have = row && left > 0;
                     copy_async<16>(put + (m * 2 + i) * 512, have ? static_cast<const void*>(w[m][i]) : span.from, have);
                 } else if (row) {
-                    const unsigned c = lane % 4;
-                    copy_chunks<W, 64>(raw + (put - base) - lane * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW,
-                                       w[m][i] - c * PER, c, span, inside);
+                    const unsigned c = lane % 4;  // w[m][i]: the lane's chunk
+                    copy_chunks<W, 64>(raw + (put - base) - (lane - c) * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW, w[m][i], c,
+                                       span, inside);
                 }
             }
     }
@@ -423,7 +425,7 @@ struct Ring {
                 }
             } else {
                 const unsigned c = lane % 4;
-                copy_chunks<X, BLOCK * sizeof(X)>(raw + (at - base) - lane * 16 + lane / 4 * XROW, x[n] - c * PER, c, span, inside);
+                copy_chunks<X, BLOCK * sizeof(X)>(raw + (at - base) - (lane - c) * 16 + lane / 4 * XROW, x[n], c, span, inside);
             }
         }
     }
@@ -617,19 +619,24 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             w_inside = x_inside = !VEC;
 #pragma unroll
             for (unsigned m = 0; m < MT; ++m) {
-                w[m][0] = static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i + m * 8) * a.H + k;
-                w[m][1] = w[m][0] + static_cast<std::size_t>(a.I) * a.H;
                 if (i + m * 8 >= a.I) continue;
                 ok |= 3u << 2 * m;
-                if (!VEC) w_inside &= is_inside<64>(w[m][0] - k, blocks, w_span) && is_inside<64>(w[m][1] - k, blocks, w_span);
+#pragma unroll
+                for (unsigned up = 0; up < 2; ++up) {
+                    const W* row = static_cast<const W*>(a.w_gate_up) +
+                                   ((static_cast<std::size_t>(e) * 2 + up) * a.I + i + m * 8) * a.H;
+                    w[m][up] = VEC ? row + k : lane_chunk(row, 64, at, c);
+                    if (!VEC) w_inside &= is_inside<64>(row, blocks, w_span);
+                }
             }
             x_ok = 0;
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
                 if (t * 8 + r < group_count(g)) {
                     x_ok |= 1u << t;
-                    x[t] = static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x + k;
-                    if (!VEC) x_inside &= is_inside<R::BLOCK * sizeof(X)>(x[t] - k, blocks, x_span);
+                    const X* row = static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x;
+                    x[t] = VEC ? row + k : lane_chunk(row, R::BLOCK * sizeof(X), at, c);
+                    if (!VEC) x_inside &= is_inside<R::BLOCK * sizeof(X)>(row, blocks, x_span);
                 }
             left = static_cast<int>(a.H) - static_cast<int>(k);
             put_left = count;
@@ -796,9 +803,10 @@ moe_down(MoeDecodeArgs a, unsigned per) {
 #pragma unroll
             for (unsigned i = 0; i < 2 * MT; ++i) {
                 const unsigned h = h0 + r + 8 * i;
-                w[i / 2][i % 2] = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I + k;
+                const W* row = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I;
+                w[i / 2][i % 2] = VEC ? row + k : lane_chunk(row, 64, put_u & (parts - 1), c);
                 if (h < a.H) ok |= 1u << i;
-                if (!VEC && h < a.H) inside &= is_inside<64>(w[i / 2][i % 2] - k, blocks, w_span);
+                if (!VEC && h < a.H) inside &= is_inside<64>(row, blocks, w_span);
             }
             x_ok = 0;
 #pragma unroll
@@ -926,17 +934,22 @@ cudaError_t launch_down(const MoeDecodeArgs& a, cudaStream_t s) {
 
 template <typename X, typename W>
 cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
-    const bool vec = a.H % 8 == 0 && a.I % kPer<W> == 0 && a.ld_x % 8 == 0 && aligned16(a.x) &&
-                     aligned16(a.w_gate_up) && aligned16(a.w_down);
-    // 16 tokens per group where the experts have more than 4 on average: fewer
-    // experts are read twice; else 8, whose smaller stages leave more weights in flight
+    // rows of 16-byte pieces, for each launch by itself
+    const bool vec_up = a.H % 8 == 0 && a.ld_x % 8 == 0 && aligned16(a.x) && aligned16(a.w_gate_up);
+    const bool vec_down = a.I % kPer<W> == 0 && aligned16(a.w_down);
+    // 16 tokens per group, and 16 rows of gate and up per item, where the
+    // experts have more than 4 tokens on average: fewer experts are read twice,
+    // fewer activations split twice (128 tokens of 4096 x 448 x 16: 87 us, with
+    // 8 rows 107); else 8 of each, whose smaller stages leave more weights in flight
     const bool wide = 2 * a.T > 4 * a.E;
-    cudaError_t e = vec ? wide ? launch_up<X, W, 2, 2, true>(a, s) : launch_up<X, W, 1, 1, true>(a, s)
-                        : wide ? launch_up<X, W, 2, 2, false>(a, s) : launch_up<X, W, 1, 1, false>(a, s);
+    cudaError_t e = vec_up ? wide ? launch_up<X, W, 2, 2, true>(a, s) : launch_up<X, W, 1, 1, true>(a, s)
+                           : wide ? launch_up<X, W, 2, 2, false>(a, s) : launch_up<X, W, 1, 1, false>(a, s);
     if (e != cudaSuccess) return e;
-    // 32 output rows per CTA as long as that reaches most SMs: the activations are read once for both tiles
-    const bool tall = a.H >= 2368;
-    if (vec) return tall ? launch_down<X, W, 2, 1, true>(a, s) : launch_down<X, W, 1, 1, true>(a, s);
+    // 32 output rows per CTA as long as that reaches most SMs: the activations
+    // are read once for both tiles, and 16 rows would leave a second round of CTAs
+    const bool tall = a.H > 16u * static_cast<unsigned>(sm_count());
+    if (vec_down) return tall ? launch_down<X, W, 2, 1, true>(a, s) : launch_down<X, W, 1, 1, true>(a, s);
+    if (tall) return wide ? launch_down<X, W, 2, 2, false>(a, s) : launch_down<X, W, 2, 1, false>(a, s);
     return wide ? launch_down<X, W, 1, 2, false>(a, s) : launch_down<X, W, 1, 1, false>(a, s);
 }
 
