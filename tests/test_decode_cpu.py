@@ -84,3 +84,16 @@ def test_host_tensors_are_refused():
     with pytest.raises(ops.InvalidArgument):
         decode.kv4_append_gpu(torch.zeros(1, 1, 64), torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32),
                               torch.zeros(1, dtype=torch.int32), cache, torch.zeros(1, 1, dtype=torch.int32))
+
+
+def test_python_calls_refuse_what_is_no_tensor_or_not_on_a_gpu():
+    import torch
+
+    x = torch.zeros(2, 8)
+    for bad in (x, None, "x"):
+        with pytest.raises(ops.InvalidArgument):
+            decode.moe_decode_gpu(bad, x, x, x.view(2, 2, 4), x, ws=decode.MoeWorkspace(2, 4, "cpu"))
+    with pytest.raises(ops.InvalidArgument):
+        decode.moe_decode_gpu(x, x, x, x.view(2, 2, 4), x)
+    with pytest.raises(TypeError):
+        decode._decode_calls.moe_decode(x)
