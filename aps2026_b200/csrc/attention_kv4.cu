@@ -11,23 +11,36 @@
 // sum p_j (m_j + 8 s_j). (A nibble left as an fp16 subnormal needs no FMA, but
 // the matrix unit aligns by the exponent field: it cost 7 bits.)
 // The other operands keep fp32's accuracy as two fp16 parts each: queries,
-// scaled by a power of two per row, as the upper and lower 8 rows of one M =
-// 16 operand; p s as two operands of one accumulator. R is raised only when
-// some p s would pass 2^15 (fp16's end), so most tiles rescale nothing.
+// scaled by a power of two per row, and p s. R is raised only when some p s
+// would pass 2^15 (fp16's end), so most steps rescale nothing. The matrix
+// unit adds to its accumulator with truncation, a bias that grows with the
+// chain; so a chain is one step long (4 instructions at most) and the steps
+// are added in registers.
 //
-// HBM bound: 144 bytes per visible position and KV head (head_dim 128). A
-// warp takes 32 positions a step from its own cp.async ring, S = Q K^T with
-// 8 query rows (heads x new tokens of one KV head), then O^T += V^T P^T; in
-// these two orders a thread's P is already the operand the second product
-// wants. The matrix unit adds to its accumulator with truncation, a bias
-// that grows with the chain; so a chain is one step long (4 instructions)
-// and the steps are added in registers.
+// A warp takes 32 positions a step from its own cp.async ring: S = Q K^T, then
+// O^T += V^T P^T. Two forms of a tile of rows (heads x new tokens of one KV
+// head): Wide, 8 rows, and Narrow, 4 rows, which a single token of a group of
+// up to 4 heads takes, and where hi and lo parts share an instruction's
+// columns (64 sequences of 4095 .. 32768 positions, 4 KV heads of 4 heads
+// each: 167 us, Wide with half of its rows empty 214).
 //
-// All (row tile, KV head) pairs' steps form one list that is cut into equal
-// shares, one per CTA, two CTAs per SM: ragged lengths and one long sequence
-// load every SM alike. A share holds the end of one pair, whole pairs, and
-// the start of another; parts meet in the workspace, where the last CTA to
-// arrive adds them in the list's order, so results repeat bit for bit.
+// The steps of all (row tile, KV head) pairs are cut into equal shares, one
+// per CTA, two CTAs per SM, so that ragged lengths and one long sequence load
+// every SM alike. When there are no more pairs than CTAs, each pair gets CTAs
+// of its own, unless that leaves some CTA with 28 steps more than its share:
+// a CTA with parts of two pairs pays a part's latencies twice (32 sequences of
+// 129 .. 4096 positions, window 2047: 18.6 us, as one list 27.2; 16 of 4095 ..
+// 32768 with 8 KV heads 117 and 113). A pair's parts
+// meet in the workspace, where the last CTA to arrive adds them in the
+// order of their keys, so results repeat bit for bit.
+//
+// What bounds it: with long contexts, instruction issue. 144 bytes per
+// position and KV head (head_dim 128) would be 105 us of HBM time for the 679
+// MB of 64 sequences; the step's some 700 instructions (half of them turn
+// nibbles into fp16) take 167 to 178 (issue 63% active, ALU 56%, matrix unit 24%,
+// DRAM 3.9 TB/s). With little work per CTA, the chain of latencies: lengths,
+// page numbers, keys, the warps' meeting, the parts' meeting (31 us for one
+// sequence of 131,069, 11.7 us of HBM time; 7 us for one of 37).
 #include <algorithm>
 #include <cmath>
 
@@ -409,7 +422,8 @@ __device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, un
            (a.window == 0 || pos - j < static_cast<int>(a.window) || j < static_cast<int>(a.sinks));
 }
 
-// Eight rows. Queries are the M = 16 operand of QK (hi parts in rows 0..7, lo
+// Eight rows (5 new tokens of 4 heads on each of 4 KV heads, 12 sequences of
+// 500 .. 4000: 27.5 us). Queries are the M = 16 operand of QK (hi parts in rows 0..7, lo
 // in 8..15), so thread (r, c) gets the scores of row r and keys 8b + 2c, + 1,
 // which is where the second product wants P^T (k = keys, n = rows).
 template <unsigned D>
@@ -1217,7 +1231,7 @@ __device__ __forceinline__ void run_part(const AttnKv4Args& a, const Part& p, Sm
 }
 
 // Each pair on CTAs of its own, as few as keep every CTA at `most` units:
-// sum over pairs of ceil(units / most) * heads CTAs. Returns the least of
+// the sum over pairs of ceil(units / most) * heads. Returns the least of
 // kWarps candidates for `most` that fits the grid (0: none does). One warp
 // tries one candidate.
 template <unsigned D>

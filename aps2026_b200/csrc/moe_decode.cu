@@ -4,28 +4,38 @@
 // Mathematics: for token t and each of its two experts e,
 //   a(t, e) = silu(Wg[e] x[t]) * (Wu[e] x[t]),   out[t] = sum_e g(t, e) Wd[e] a(t, e).
 //
-// HBM bound: with T <= 128 tokens every weight of an expert that is reached
-// is read once and meets few tokens, so the weights stream from HBM through a
-// ring of cp.async stages in shared memory. Which k a lane holds of the
-// matrix instruction's M = 16 operand is free as long as both operands agree,
-// so a lane takes 16 neighbouring bytes of its rows: it copies exactly what
-// it will use, every ring is private to a lane, and no barrier is needed. Up
-// to 16 tokens are the instruction's N, staged the same way.
-// The instruction multiplies bf16 or TF32; fp32's accuracy is kept in
-// parts: bf16 weights meet fp32 activations as three bf16 parts (24 bits),
-// fp32 weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
+// The weights stream from HBM once (groups of one expert read them again, from
+// L2) and meet few tokens. Which k a lane holds of the matrix instruction's
+// M = 16 operand is free as long as both operands agree, so a lane takes 16
+// neighbouring bytes of its rows: it copies exactly what it will use, through
+// its own ring of cp.async stages in shared memory, without barriers. The
+// tokens are the instruction's N, staged the same way. Rows that start at any
+// element cannot be copied so: their 16-byte chunks are brought by the row's
+// four lanes and read across them, shifted (H = 1001, I = 333, 128 tokens: 61
+// -> 45 us against loading them word by word).
+// The instruction multiplies bf16 or TF32; fp32's accuracy is kept in parts:
+// bf16 weights meet fp32 activations as three bf16 parts (24 bits), fp32
+// weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
 // truncates, so chains are short (2 blocks) and added in registers.
 //
-// Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens, 8
-// rows of gate and the same of up); a CTA takes equally many items, one
-// after the other through the same rings. Its warps interleave the k blocks,
-// so together they read whole lines, and add up in shared memory. It leaves
-// the activations in their parts. Launch 2, moe_down: CTA = 16 MT rows of the
-// output for all tokens; warps take (expert, 8 NT of its tokens, part of k) and
-// meet in shared memory, where a token's two experts are summed in ascending
-// order: no float atomics, results repeat. Each CTA routes for itself (T x E
-// logits). Launch 2 starts under launch 1 and has routed and requested its
-// first weights before it waits.
+// Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens,
+// 8 MT rows of gate and the same of up); a CTA takes equally many items, one
+// after the other through the same rings. The warps of an item interleave its
+// k blocks, so together they read whole lines, and add up in shared memory.
+// It leaves the activations in their parts. Launch 2, moe_down: CTA = 16 MT
+// rows of the output for its tokens; warps take (expert, 8 NT of its tokens,
+// part of k) and meet in shared memory, where a token's two experts are
+// summed in ascending order: no float atomics, results repeat. Each CTA
+// routes for itself (T x E logits). Launch 2 starts under launch 1 and has
+// routed and requested its first weights before it waits.
+//
+// What bounds it: one token, the two launches' latencies (routing, first
+// weights, the meeting, the hand-over: 13 us at 4096 x 448 x 16 in bf16,
+// 3.4 us of HBM time). 9 tokens, HBM with those latencies (28 us, 19 of HBM
+// time). 61 tokens in fp32, instruction issue: splitting weights into TF32
+// parts and three products each (launch 1: 64 us, issue 55% active, matrix
+// unit 31%, no stall on memory; both 92, HBM time 55). 128 tokens, splitting
+// the activations anew for every 16 rows (45 us at 1001 x 333 x 7).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -40,7 +50,7 @@ constexpr unsigned kMaxGroups = kMaxExperts + 2 * kMaxDecodeTokens / 8;
 constexpr unsigned kChain = 2;           // blocks between two additions in registers
 constexpr unsigned kDownPartials = 256;  // (part of k, assignment) sums of moe_down
 constexpr unsigned kWarps = 16;          // one CTA per SM: all its shared memory is rings
-constexpr unsigned kRing = 11264;        // bytes of a warp's stages
+constexpr unsigned kRing = 11264;        // bytes of a warp's stages: 16 rings, the sums and the plan fill 227 KB
 
 struct MoeDecodeArgs {
     const void* x;

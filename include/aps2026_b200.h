@@ -376,7 +376,8 @@ int b2_add(float* a, const float* b, size_t n, b2_stream_t stream);
  * the value held is s * c + m.
  * page_size: a power of two, 8 at least; head_dim 64 or 128; data 16-byte
  * aligned, pages * b2_kv4_page_bytes long; pages and page_table in device
- * memory.
+ * memory. page_size up to 2^20, a page below 4 GB; pages, seqs and
+ * max_pages below 2^32 - 1.
  */
 typedef struct b2_kv4_cache {
     void* data;
@@ -446,6 +447,9 @@ int b2_kv4_read(const b2_kv4_cache* cache, const uint32_t* row_seq,
  * workspace: b2_attention_kv4_workspace_size bytes, 16-byte aligned, all zero
  * before its first use; every call leaves it ready for the next. Calls that
  * overlap on the GPU must not share it.
+ * Limits: max_len <= 2^28; max_queries * q_heads < 2^31; with up to 8 query
+ * rows of a KV head per row tile, seqs * tiles * kv_heads * max_len < 2^35.
+ * scale must be finite; 0 and below are allowed.
  * Reported through b2_device_status (B2_CHECK_KV4): a sequence with more
  * than max_queries query rows or offsets outside [0, rows] (its rows are not
  * written); a length above max_len or the table's reach (its rows are zero);
@@ -473,7 +477,8 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride,
  *            w_down[e] (silu(w_gate_up[e][:I] x[t]) * (w_gate_up[e][I:] x[t]))
  * x [T, ld_x >= H] and out [T, ld_out >= H]: x_dtype; logits [T, E] fp32,
  * 2 <= E <= 32; w_gate_up [E, 2I, H] and w_down [E, H, I] contiguous:
- * w_dtype. Sums in fp32; the products are those of the inputs as they are.
+ * w_dtype, aligned to their element at least (rows and tensors aligned to 16
+ * bytes are faster). Sums in fp32; fp32 operands keep 22 bits or more.
  * out may not overlap x. T > 128: B2_ERR_UNSUPPORTED (route with
  * b2_moe_route and run the experts as grouped products).
  * workspace: b2_moe_decode_workspace_size bytes, 16-byte aligned; no
