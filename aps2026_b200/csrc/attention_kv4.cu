@@ -950,7 +950,7 @@ __device__ __forceinline__ void place_query(const AttnKv4Args& a, const float (&
     for (unsigned g = 0; g < G; ++g) sum[g] = warp_sum(sum[g]);
     // 2^e with top * 2^e in [2^9, 2^10)
     int e = 136 - static_cast<int>(__float_as_uint(top) >> 23);
-    e = top == 0.0f ? 0 : max(-100, min(e, 100));
+    e = top == 0.0f ? 0 : max(-118, min(e, 100));
     const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
     if (lane == 0) {
         // positive, so that a masked score stays -inf
