@@ -1215,15 +1215,16 @@ __device__ __forceinline__ void run_part(const AttnKv4Args& a, const Part& p, Sm
     const std::size_t slot = static_cast<std::size_t>(2) * blockIdx.x + (p.from == 0 ? 1 : 0);
     run_segment<T, D, Rows>(a, t, seq, p.head, p.from, p.to, p.n == 1, slot, sm);
     if (p.n > 1) {
-        __threadfence();
+        // releases the CTA's parts (through the barrier), acquires the others'
         __syncthreads();
         if (threadIdx.x == 0) {
-            sm.last = atomicAdd(a.counters + p.first, 1u) == p.n - 1;
+            unsigned before;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + p.first) : "memory");
+            sm.last = before == p.n - 1;
             if (sm.last) a.counters[p.first] = 0;
         }
         __syncthreads();
         if (sm.last) {
-            __threadfence();
             join_parts<T, D>(a, t, p.head, p.first, p.n, sm);
         }
     }
