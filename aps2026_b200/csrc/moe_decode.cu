@@ -16,7 +16,9 @@
 // The instruction multiplies bf16 or TF32; fp32's accuracy is kept in parts:
 // bf16 weights meet fp32 activations as three bf16 parts (24 bits), fp32
 // weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
-// truncates, so chains are short (2 blocks) and added in registers.
+// truncates, a bias that grows with the chain, so a chain is one block long
+// and blocks are added in registers (61 tokens in fp32: error 6.5e-7 of the
+// output and 84 us; two blocks per chain 9.6e-7 and 88).
 //
 // Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens,
 // 8 MT rows of gate and the same of up); a CTA takes equally many items, one
@@ -47,7 +49,6 @@ namespace {
 
 constexpr unsigned kMaxDecodeTokens = 128;
 constexpr unsigned kMaxGroups = kMaxExperts + 2 * kMaxDecodeTokens / 8;
-constexpr unsigned kChain = 2;           // blocks between two additions in registers
 constexpr unsigned kDownPartials = 256;  // (part of k, assignment) sums of moe_down
 constexpr unsigned kWarps = 16;          // one CTA per SM: all its shared memory is rings
 constexpr unsigned kRing = 11264;        // bytes of a warp's stages: 16 rings, the sums and the plan fill 227 KB
@@ -331,6 +332,13 @@ struct Skew {
     int left;  // elements from the lane's k to the rows' ends
 };
 
+template <unsigned NT, unsigned MT>
+__device__ __forceinline__ void clear(float (&v)[NT][MT][4]) {
+#pragma unroll
+    for (unsigned n = 0; n < NT; ++n)
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) v[n][m][0] = v[n][m][1] = v[n][m][2] = v[n][m][3] = 0.0f;
+}
 // The stages of one warp: MT 16-row tiles of a weight block (lane's rows r and
 // r + 8 of each) and NT 8-token tiles of activations (lane's token r). VEC:
 // every 16 bytes of a row of weights (XVEC: the activations that meet them)
@@ -440,8 +448,8 @@ struct Ring {
         }
     }
 
-    // part[n] += the stage's products for nt token tiles.
-    __device__ __forceinline__ void multiply(unsigned nt, float (&part)[NT][MT][4], unsigned lane,
+    // acc[n] += the stage's products for nt token tiles.
+    __device__ __forceinline__ void multiply(unsigned nt, float (&acc)[NT][MT][4], unsigned lane,
                                              const Skew<MT, NT>& skew) {
         constexpr unsigned PARTS = PLANES ? PLANES : kParts<X, W>;
         uint4 w[MT][2];
@@ -508,13 +516,15 @@ struct Ring {
                 b[0][0] = v[0] << 16; b[0][1] = v[0] & 0xFFFF0000u;
                 b[0][2] = v[1] << 16; b[0][3] = v[1] & 0xFFFF0000u;
             }
+            float part[1][MT][4];  // of this block alone
+            clear(part);
             if constexpr (sizeof(W) == 2) {
 #pragma unroll
                 for (unsigned q = PARTS; q-- > 0;)
 #pragma unroll
                     for (unsigned m = 0; m < MT; ++m) {
-                        mma_bf16(part[n][m], w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, b[q][0], b[q][1]);
-                        mma_bf16(part[n][m], w[m][0].z, w[m][1].z, w[m][0].w, w[m][1].w, b[q][2], b[q][3]);
+                        mma_bf16(part[0][m], w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, b[q][0], b[q][1]);
+                        mma_bf16(part[0][m], w[m][0].z, w[m][1].z, w[m][0].w, w[m][1].w, b[q][2], b[q][3]);
                     }
             } else {
 #pragma unroll
@@ -533,35 +543,20 @@ struct Ring {
                     }
 #pragma unroll
                     for (unsigned i = 0; i < 4; i += 2) {
-                        mma_tf32(part[n][m], l0[i], l1[i], l0[i + 1], l1[i + 1], b[0][i], b[0][i + 1]);
+                        mma_tf32(part[0][m], l0[i], l1[i], l0[i + 1], l1[i + 1], b[0][i], b[0][i + 1]);
                         if (PARTS == 2)
-                            mma_tf32(part[n][m], h0[i], h1[i], h0[i + 1], h1[i + 1], b[PARTS - 1][i], b[PARTS - 1][i + 1]);
-                        mma_tf32(part[n][m], h0[i], h1[i], h0[i + 1], h1[i + 1], b[0][i], b[0][i + 1]);
+                            mma_tf32(part[0][m], h0[i], h1[i], h0[i + 1], h1[i + 1], b[PARTS - 1][i], b[PARTS - 1][i + 1]);
+                        mma_tf32(part[0][m], h0[i], h1[i], h0[i + 1], h1[i + 1], b[0][i], b[0][i + 1]);
                     }
                 }
             }
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m)
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) acc[n][m][i] += part[0][m][i];
         }
     }
 };
-
-template <unsigned NT, unsigned MT>
-__device__ __forceinline__ void clear(float (&v)[NT][MT][4]) {
-#pragma unroll
-    for (unsigned n = 0; n < NT; ++n)
-#pragma unroll
-        for (unsigned m = 0; m < MT; ++m) v[n][m][0] = v[n][m][1] = v[n][m][2] = v[n][m][3] = 0.0f;
-}
-// acc += part, part = 0.
-template <unsigned NT, unsigned MT>
-__device__ __forceinline__ void flush(float (&acc)[NT][MT][4], float (&part)[NT][MT][4]) {
-#pragma unroll
-    for (unsigned n = 0; n < NT; ++n)
-#pragma unroll
-        for (unsigned m = 0; m < MT; ++m)
-#pragma unroll
-            for (unsigned i = 0; i < 4; ++i) acc[n][m][i] += part[n][m][i];
-    clear(part);
-}
 
 // ---- launch 1 ---------------------------------------------------------------------------
 
@@ -677,9 +672,8 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
         const unsigned item = (set << shift) + mine;
         if (item < items) {
             const unsigned g = sm.plan.group[item / tiles], n = group_count(g), nt = (n + 7) / 8;
-            float acc[NT][MT][4], part[NT][MT][4];
+            float acc[NT][MT][4];
             clear(acc);
-            clear(part);
             Skew<MT, NT> skew{};
             if constexpr (!VEC) {
                 const unsigned e = group_expert(g), i = item % tiles * U::ROWS + r;
@@ -701,12 +695,10 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                 cp_async_commit();
                 cp_async_wait<R::STAGES - 1>();
                 R::meet();
-                ring.multiply(nt, part, lane, skew);
+                ring.multiply(nt, acc, lane, skew);
                 skew.left -= static_cast<int>(step);
                 R::step(ring.get, ring.base);
-                if (i % kChain == kChain - 1) flush(acc, part);
             }
-            flush(acc, part);
 #pragma unroll
             for (unsigned t = 0; t < NT; ++t)
                 if (t < nt)
@@ -862,9 +854,8 @@ moe_down(MoeDecodeArgs a, unsigned per) {
     for (unsigned u = warp; u < units; u += kWarps) {
         const unsigned g = sm.plan.group[u >> shift], n = group_count(g);
         const unsigned count = blocks_of(u);
-        float acc[NT][MT][4], part[NT][MT][4];
+        float acc[NT][MT][4];
         clear(acc);
-        clear(part);
         Skew<MT, NT> skew{};
         if constexpr (!VEC) {
 #pragma unroll
@@ -879,12 +870,10 @@ moe_down(MoeDecodeArgs a, unsigned per) {
             cp_async_commit();
             cp_async_wait<R::STAGES - 1>();
             R::meet();
-            ring.multiply((n + 7) / 8, part, lane, skew);
+            ring.multiply((n + 7) / 8, acc, lane, skew);
             skew.left -= static_cast<int>(parts * R::BLOCK);
             R::step(ring.get, ring.base);
-            if (b % kChain == kChain - 1) flush(acc, part);
         }
-        flush(acc, part);
 #pragma unroll
         for (unsigned t = 0; t < 2 * NT; ++t) {
             const unsigned at = t / 2 * 8 + 2 * c + t % 2;
