@@ -11,8 +11,8 @@
 // its own ring of cp.async stages in shared memory, without barriers. The
 // tokens are the instruction's N, staged the same way. Rows that start at any
 // element cannot be copied so: their 16-byte chunks are brought by the row's
-// four lanes and read across them, shifted (H = 1001, I = 333, 128 tokens: 61
-// -> 45 us against loading them word by word).
+// four lanes and read across them, shifted (H = 1001, I = 333, 128 tokens: 49
+// us against 61 word by word, before the other steps).
 // The instruction multiplies bf16 or TF32; fp32's accuracy is kept in parts:
 // bf16 weights meet fp32 activations as three bf16 parts (24 bits), fp32
 // weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
@@ -32,12 +32,12 @@
 // routed and requested its first weights before it waits.
 //
 // What bounds it: one token, the two launches' latencies (routing, first
-// weights, the meeting, the hand-over: 13 us at 4096 x 448 x 16 in bf16,
-// 3.4 us of HBM time). 9 tokens, HBM with those latencies (28 us, 19 of HBM
+// weights, the meeting, the hand-over: 12.4 us at 4096 x 448 x 16 in bf16,
+// 3.4 us of HBM time). 9 tokens, HBM with those latencies (27 us, 19 of HBM
 // time). 61 tokens in fp32, instruction issue: splitting weights into TF32
 // parts and three products each (launch 1: 64 us, issue 55% active, matrix
-// unit 31%, no stall on memory; both 92, HBM time 55). 128 tokens, splitting
-// the activations anew for every 16 rows (45 us at 1001 x 333 x 7).
+// unit 31%, no stall on memory; both 87, HBM time 55). 128 tokens, splitting
+// the activations anew for every 16 rows (44 us at 1001 x 333 x 7).
 #include <algorithm>
 
 #include <cuda_bf16.h>
