@@ -11,9 +11,8 @@
 // its own ring of cp.async stages in shared memory, without barriers. The
 // tokens are the instruction's N, staged the same way. Rows that start at any
 // element cannot be copied so: their 16-byte chunks are brought by the row's
-// four lanes, as asynchronously, and read across them, shifted. It costs a
-// block 267 instructions where an aligned one takes 160 (5 tokens of 2944 x
-// 201 and of 3001 x 201: launch 1 14 and 24 us).
+// four lanes, as asynchronously, and read across them, shifted (5 tokens of
+// 3001 x 201 28 us; of 2944 x 201, where only launch 2 has such rows, 21).
 // The instruction multiplies bf16 or TF32; fp32's accuracy is kept in parts:
 // bf16 weights meet fp32 activations as three bf16 parts (24 bits), fp32
 // weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
@@ -38,7 +37,7 @@
 // time). 61 tokens in fp32, instruction issue: splitting weights into TF32
 // parts and three products each (launch 1: 64 us, issue 55% active, matrix
 // unit 31%, no stall on memory; both 87, HBM time 55). 128 tokens, splitting
-// the activations anew for every 16 rows (44 us at 1001 x 333 x 7).
+// the activations anew for every 16 rows (41 us at 1001 x 333 x 7).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -257,11 +256,9 @@ __device__ __forceinline__ void split_tf32(unsigned w, unsigned& hi, unsigned& l
 }
 
 // Where a row that starts at any element lies in a stage: the 16-byte chunks
-// of memory that its block touches, side by side. They are brought by the four
-// lanes of the row and read across them from byte `skip` on.
-struct Span {
-    const unsigned char *from, *to;  // the tensor: nothing is read outside
-};
+// of memory that its block touches, side by side, zeros past the row's end.
+// They are brought by the four lanes of the row and read across them from byte
+// `skip` on.
 template <typename T>
 __device__ __forceinline__ unsigned skip_of(const T* row) {
     return static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(row)) & 15u;
@@ -269,19 +266,15 @@ __device__ __forceinline__ unsigned skip_of(const T* row) {
 __device__ __forceinline__ const unsigned char* chunk_of(const void* p) {
     return reinterpret_cast<const unsigned char*>(reinterpret_cast<std::uintptr_t>(p) & ~std::uintptr_t(15));
 }
-// Whether all chunks of a row's `blocks` blocks of BYTES bytes are inside the tensor.
-template <unsigned BYTES>
-__device__ __forceinline__ bool is_inside(const void* row, unsigned blocks, const Span& span) {
-    const unsigned char* first = chunk_of(row);
-    return first >= span.from && first + (static_cast<std::size_t>(blocks) * BYTES + 16) <= span.to;
-}
 // Lane c's share of a block of BYTES bytes and of the chunks around them:
 // chunks c, c + 4, ... of the row's, the first of which is at `chunk` and goes
-// to `dst`. inside: the tensor holds all of them.
+// to `dst`. there: bytes from `chunk` to the row's end. whole: all the chunks
+// are inside the tensor, which begins at `tensor`, and before the row's end.
 template <typename T, unsigned BYTES>
-__device__ __forceinline__ void copy_chunks(unsigned char* dst, const void* chunk, unsigned c, const Span& span, bool inside) {
+__device__ __forceinline__ void copy_chunks(unsigned char* dst, const void* chunk, unsigned c, const void* tensor, int there,
+                                            bool whole) {
     const unsigned char* from = static_cast<const unsigned char*>(chunk);
-    if (inside) {
+    if (whole) {
         const unsigned to = smem_addr(dst);
 #pragma unroll
         for (unsigned i = 0; i < BYTES / 16 + 1; i += 4)
@@ -290,17 +283,16 @@ __device__ __forceinline__ void copy_chunks(unsigned char* dst, const void* chun
         return;
     }
 #pragma unroll 1
-    for (unsigned i = 0; i + c <= BYTES / 16; i += 4, from += 64, dst += 64) {
-        if (from >= span.from) {
-            const std::ptrdiff_t there = span.to - from;
-            const int bytes = there >= 16 ? 16 : there > 0 ? static_cast<int>(there) : 0;
+    for (unsigned i = 0; i + c <= BYTES / 16; i += 4, from += 64, dst += 64, there -= 64) {
+        const int bytes = max(0, min(there, 16));
+        if (from >= tensor || bytes == 0) {
             asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)),
-                         "l"(bytes ? from : chunk_of(span.from) + 16), "r"(bytes)
+                         "l"(bytes ? from : chunk_of(tensor) + 16), "r"(bytes)
                          : "memory");
         } else {  // a tensor that starts inside a chunk
-            for (unsigned e = 0; e < 16; e += sizeof(T))
+            for (int e = 0; e < 16; e += sizeof(T))
                 *reinterpret_cast<T*>(dst + e) =
-                    from + e >= span.from && from + e < span.to ? *reinterpret_cast<const T*>(from + e) : T(0.0f);
+                    from + e >= tensor && e < bytes ? *reinterpret_cast<const T*>(from + e) : T(0.0f);
         }
     }
 }
@@ -309,9 +301,9 @@ template <typename T>
 __device__ __forceinline__ const T* lane_chunk(const T* row, unsigned block_bytes, unsigned at, unsigned c) {
     return reinterpret_cast<const T*>(chunk_of(row) + (static_cast<std::size_t>(at) * block_bytes + c * 16));
 }
-// Lane c's WORDS words of a row in a stage; elements from `left` on are zeros.
+// Lane c's WORDS words of a row in a stage.
 template <typename T, unsigned WORDS>
-__device__ __forceinline__ void read_skewed(unsigned row, unsigned skip, unsigned c, int left, unsigned (&v)[WORDS]) {
+__device__ __forceinline__ void read_skewed(unsigned row, unsigned skip, unsigned c, unsigned (&v)[WORDS]) {
     const unsigned at = row + (skip & 12u) + c * WORDS * 4;
     unsigned w[WORDS + 1];
 #pragma unroll
@@ -319,18 +311,11 @@ __device__ __forceinline__ void read_skewed(unsigned row, unsigned skip, unsigne
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + i * 4));
 #pragma unroll
     for (unsigned i = 0; i < WORDS; ++i) v[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (skip & 2u) * 8) : w[i];
-    constexpr int PER_WORD = 4 / sizeof(T);
-    if (left < static_cast<int>(WORDS) * PER_WORD)
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(WORDS); ++i)
-            if (left <= i * PER_WORD) v[i] = 0;
-            else if (PER_WORD == 2 && left == i * PER_WORD + 1) v[i] &= 0xFFFFu;
 }
-// What reading needs to know of the rows that it reads.
+// skip_of the lane's rows.
 template <unsigned MT, unsigned NT>
 struct Skew {
     unsigned w[MT][2], x[NT];
-    int left;  // elements from the lane's k to the rows' ends
 };
 
 template <unsigned NT, unsigned MT>
@@ -404,8 +389,8 @@ struct Ring {
     }
     // w[m][i]: the lane's weights (row's start + k); ok: bit 2m + i set where
     // the row is there; left: weights from k to the row's end, if positive.
-    __device__ __forceinline__ void put_weights(const W* const (&w)[MT][2], unsigned ok, int left, const Span& span,
-                                                bool inside, unsigned lane) {
+    __device__ __forceinline__ void put_weights(const W* const (&w)[MT][2], unsigned ok, int left, const W* tensor,
+                                                const Skew<MT, NT>& skew, bool inside, unsigned lane) {
 #pragma unroll
         for (unsigned m = 0; m < MT; ++m)
 #pragma unroll
@@ -413,18 +398,19 @@ struct Ring {
                 const bool row = (ok >> (2 * m + i)) & 1u;
                 if (VEC) {
                     const bool have = row && left > 0;
-                    copy_async<16>(put + (m * 2 + i) * 512, have ? static_cast<const void*>(w[m][i]) : span.from, have);
+                    copy_async<16>(put + (m * 2 + i) * 512, have ? w[m][i] : tensor, have);
                 } else if (row) {
                     const unsigned c = lane % 4;  // w[m][i]: the lane's chunk
+                    const int rest = (left + static_cast<int>(c * PER)) * static_cast<int>(sizeof(W));  // of the row, from the block on
                     copy_chunks<W, 64>(raw + (put - base) - (lane - c) * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW, w[m][i], c,
-                                       span, inside);
+                                       tensor, rest + static_cast<int>(skew.w[m][i] - c * 16), inside && rest >= 80);
                 }
             }
     }
     // x[n]: the lane's activations of token tile n (of the first plane); x_ok:
     // bit n set where there is a token.
     __device__ __forceinline__ void put_acts(const X* const (&x)[NT], unsigned x_ok, int left, unsigned lane,
-                                             std::size_t plane, const Span& span, bool inside) {
+                                             std::size_t plane, const X* tensor, const Skew<MT, NT>& skew, bool inside) {
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
             if (!((x_ok >> n) & 1u)) continue;
@@ -444,7 +430,10 @@ struct Ring {
                 }
             } else {
                 const unsigned c = lane % 4;
-                copy_chunks<X, BLOCK * sizeof(X)>(raw + (at - base) - (lane - c) * 16 + lane / 4 * XROW, x[n], c, span, inside);
+                const int rest = (left + static_cast<int>(c * PER)) * static_cast<int>(sizeof(X));
+                copy_chunks<X, BLOCK * sizeof(X)>(raw + (at - base) - (lane - c) * 16 + lane / 4 * XROW, x[n], c, tensor,
+                                                  rest + static_cast<int>(skew.x[n] - c * 16),
+                                                  inside && rest >= static_cast<int>(BLOCK * sizeof(X) + 16));
             }
         }
     }
@@ -463,7 +452,7 @@ struct Ring {
 #pragma unroll
                 for (unsigned i = 0; i < 2; ++i) {
                     unsigned v[4];
-                    read_skewed<W>(get - lane * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW, skew.w[m][i], lane % 4, skew.left, v);
+                    read_skewed<W>(get - lane * 16 + ((m * 2 + i) * 8 + lane / 4) * WROW, skew.w[m][i], lane % 4, v);
                     w[m][i] = make_uint4(v[0], v[1], v[2], v[3]);
                 }
             }
@@ -475,7 +464,7 @@ struct Ring {
             unsigned v[PLANES ? 1 : XB / 4];  // raw activations
             if constexpr (PLANES == 0) {
                 if constexpr (!XVEC) {
-                    read_skewed<X>(at - lane * 16 + lane / 4 * XROW, skew.x[n], lane % 4, skew.left, v);
+                    read_skewed<X>(at - lane * 16 + lane / 4 * XROW, skew.x[n], lane % 4, v);
                 } else if constexpr (XB == 8) {
                     const uint2 y = lds8(at - lane * 8);
                     v[0] = y.x; v[1] = y.y;
@@ -606,13 +595,11 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
     const unsigned count = blocks > at ? (blocks - at + team - 1) / team : 0u;  // of a warp, per item
     R ring;
     ring.init(sm.ring[warp], lane);
-    const auto bytes = [](const void* p) { return static_cast<const unsigned char*>(p); };
-    const Span w_span{bytes(a.w_gate_up), bytes(static_cast<const W*>(a.w_gate_up) + std::size_t(2) * a.E * a.I * a.H)};
-    const Span x_span{bytes(a.x), bytes(static_cast<const X*>(a.x) + (a.T - 1) * a.ld_x + a.H)};
     // the end that fills
     unsigned put_set = blockIdx.x, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
     bool w_inside = false, x_inside = false;
+    Skew<MT, NT> put_skew{};
     const W* w[MT][2] = {};
     const X* x[NT] = {};
     const auto put_step = [&]() {
@@ -632,7 +619,8 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                     const W* row = static_cast<const W*>(a.w_gate_up) +
                                    ((static_cast<std::size_t>(e) * 2 + up) * a.I + i + m * 8) * a.H;
                     w[m][up] = VEC ? row + k : lane_chunk(row, 64, at, c);
-                    if (!VEC) w_inside &= is_inside<64>(row, blocks, w_span);
+                    put_skew.w[m][up] = skip_of(row);
+                    if (!VEC) w_inside &= chunk_of(row) >= a.w_gate_up;
                 }
             }
             x_ok = 0;
@@ -642,7 +630,8 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                     x_ok |= 1u << t;
                     const X* row = static_cast<const X*>(a.x) + (sm.plan.lists[e][group_first(g) + t * 8 + r] / 2) * a.ld_x;
                     x[t] = VEC ? row + k : lane_chunk(row, R::BLOCK * sizeof(X), at, c);
-                    if (!VEC) x_inside &= is_inside<R::BLOCK * sizeof(X)>(row, blocks, x_span);
+                    put_skew.x[t] = skip_of(row);
+                    if (!VEC) x_inside &= chunk_of(row) >= a.x;
                 }
             left = static_cast<int>(a.H) - static_cast<int>(k);
             put_left = count;
@@ -651,8 +640,8 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
         if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
             if constexpr (VEC) ring.put_whole(w, ok, true, x, x_ok, true, lane, 0);
         } else {
-            ring.put_weights(w, ok, left, w_span, w_inside, lane);
-            ring.put_acts(x, x_ok, left, lane, 0, x_span, x_inside);
+            ring.put_weights(w, ok, left, static_cast<const W*>(a.w_gate_up), put_skew, w_inside, lane);
+            ring.put_acts(x, x_ok, left, lane, 0, static_cast<const X*>(a.x), put_skew, x_inside);
         }
         R::step(ring.put, ring.base);
 #pragma unroll
@@ -688,7 +677,6 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                 for (unsigned t = 0; t < NT; ++t)
                     if (t * 8 + r < n)
                         skew.x[t] = skip_of(static_cast<const X*>(a.x) + sm.plan.lists[e][group_first(g) + t * 8 + r] / 2 * a.ld_x);
-                skew.left = static_cast<int>(a.H) - static_cast<int>(at * R::BLOCK + c * R::PER);
             }
             for (unsigned i = 0; i < count; ++i) {
                 R::meet();
@@ -697,7 +685,6 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
                 cp_async_wait<R::STAGES - 1>();
                 R::meet();
                 ring.multiply(nt, acc, lane, skew);
-                skew.left -= static_cast<int>(step);
                 R::step(ring.get, ring.base);
             }
 #pragma unroll
@@ -786,14 +773,12 @@ moe_down(MoeDecodeArgs a, unsigned per) {
     const std::size_t plane = static_cast<std::size_t>(2) * a.T * a.act_ld;
     R ring;
     ring.init(sm.ring[warp], lane);
-    const Span w_span{static_cast<const unsigned char*>(a.w_down),
-                      reinterpret_cast<const unsigned char*>(static_cast<const W*>(a.w_down) + std::size_t(a.E) * a.H * a.I)};
-
     // The warp's blocks are those of its units u = warp, warp + kWarps, ...,
     // one after the other through the ring.
     unsigned put_u = warp, put_left = 0, ok = 0, x_ok = 0;
     int left = 0;
     bool inside = false;
+    Skew<MT, NT> put_skew{};
     const W* w[MT][2] = {};
     const Act* x[NT] = {};
     const auto put_step = [&](bool with_weights, bool with_acts) {
@@ -809,7 +794,8 @@ moe_down(MoeDecodeArgs a, unsigned per) {
                 const W* row = static_cast<const W*>(a.w_down) + (static_cast<std::size_t>(e) * a.H + h) * a.I;
                 w[i / 2][i % 2] = VEC ? row + k : lane_chunk(row, 64, put_u & (parts - 1), c);
                 if (h < a.H) ok |= 1u << i;
-                if (!VEC && h < a.H) inside &= is_inside<64>(row, blocks, w_span);
+                put_skew.w[i / 2][i % 2] = skip_of(row);
+                if (!VEC && h < a.H) inside &= chunk_of(row) >= a.w_down;
             }
             x_ok = 0;
 #pragma unroll
@@ -826,9 +812,9 @@ moe_down(MoeDecodeArgs a, unsigned per) {
         if (VEC && left >= static_cast<int>(R::BLOCK - c * R::PER)) {
             if constexpr (VEC) ring.put_whole(w, ok, with_weights, x, x_ok, with_acts, lane, plane);
         } else {
-            if (with_weights) ring.put_weights(w, ok, left, w_span, inside, lane);
+            if (with_weights) ring.put_weights(w, ok, left, static_cast<const W*>(a.w_down), put_skew, inside, lane);
             // past I the row is padded with zeros to act_ld
-            if (with_acts) ring.put_acts(x, x_ok, static_cast<int>(a.act_ld - a.I) + left, lane, plane, w_span, false);
+            if (with_acts) ring.put_acts(x, x_ok, static_cast<int>(a.act_ld - a.I) + left, lane, plane, nullptr, put_skew, false);
         }
         R::step(ring.put, ring.base);
 #pragma unroll
@@ -863,7 +849,6 @@ moe_down(MoeDecodeArgs a, unsigned per) {
             for (unsigned i = 0; i < 2 * MT; ++i)
                 skew.w[i / 2][i % 2] = skip_of(static_cast<const W*>(a.w_down) +
                                                (static_cast<std::size_t>(group_expert(g)) * a.H + h0 + r + 8 * i) * a.I);
-            skew.left = static_cast<int>(a.I) - static_cast<int>((u & (parts - 1)) * R::BLOCK + c * R::PER);
         }
         for (unsigned b = 0; b < count; ++b) {
             R::meet();
@@ -872,7 +857,6 @@ moe_down(MoeDecodeArgs a, unsigned per) {
             cp_async_wait<R::STAGES - 1>();
             R::meet();
             ring.multiply((n + 7) / 8, acc, lane, skew);
-            skew.left -= static_cast<int>(parts * R::BLOCK);
             R::step(ring.get, ring.base);
         }
 #pragma unroll
