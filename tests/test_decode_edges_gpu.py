@@ -100,3 +100,22 @@ def test_attention_refuses(cuda):
         decode.attention_kv4_gpu(**{**ok, "max_queries": 1.5})
     decode.attention_kv4_gpu(**ok)
     assert bool(ok["out"].isfinite().all()) and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_heads", [4, 16])
+def test_attention_queries_of_any_size(cuda, q_heads):
+    """Queries times 2^k at a scale of 2^-k are the same queries, bit for bit."""
+    import torch
+
+    from aps2026_b200 import decode
+
+    g, n = _gen(q_heads + 7), 333
+    cache, table, _, _ = _filled(g, [n], 16, 2, 64)
+    q, lens = _randn(g, 1, q_heads, 64), torch.tensor([n], dtype=torch.int32, device="cuda")
+    want = torch.empty_like(q)
+    decode.attention_kv4_gpu(q, cache, table, lens, want, scale=0.125)
+    assert bool(want.isfinite().all())
+    for k in (-90, 60, 115):
+        out = torch.empty_like(q)
+        decode.attention_kv4_gpu(q * 2.0 ** k, cache, table, lens, out, scale=0.125 * 2.0 ** -k)
+        assert torch.equal(out, want), k
