@@ -1261,6 +1261,7 @@ attention_kv4_shares(AttnKv4Args a) {
         return (make_tile<Rows::ROWS>(a, pair / a.tiles, pair % a.tiles, false).total + kStep - 1) / kStep;
     };
 
+    if (threadIdx.x == 0) sm.found_pair = pairs;  // none yet
     // ---- sizes of all pairs; rows that see nothing are written here ----
     unsigned all_units = 0;  // the entry point sees to it that sums fit 32 bits
     unsigned units = 0, before = 0, total = 0;  // of pair threadIdx.x, when there are up to kPairCache
@@ -1279,6 +1280,7 @@ attention_kv4_shares(AttnKv4Args a) {
         all_units += total;
     }
     const unsigned work = all_units * heads;
+    if (work == 0) return;  // no row sees a key: their zeros are written, and nothing is to be shared out
     // short contexts: not less than a pair, up to a unit per warp, so that a
     // pair is not cut for nothing
     const unsigned share = max((work + gridDim.x - 1) / gridDim.x, min((all_units + pairs - 1) / pairs, kWarps));
@@ -1340,6 +1342,7 @@ attention_kv4_shares(AttnKv4Args a) {
         if (!most) {  // the list's part at unit `at`
             unsigned size = 0;
             for (;; ++part.pair) {  // skips pairs that see nothing
+                if (part.pair >= pairs) return;  // lens changed under the call
                 size = part.pair - block0 < kPairCache ? sm.pair_units[part.pair - block0] : units_of(part.pair);
                 if (at < (pair_begin + size) * heads) break;
                 pair_begin += size;

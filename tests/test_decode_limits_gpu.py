@@ -1,0 +1,75 @@
+"""The decode operators at the ends of what they take: batches in which no row
+sees a key, and the largest and smallest numbers."""
+import math
+
+import pytest
+
+from test_decode_edges_gpu import _filled
+from test_decode_gpu import _gen, _i32, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("seqs,kv_heads,q_heads", [(3, 2, 8), (128, 4, 16), (300, 1, 8), (300, 4, 4)])
+@pytest.mark.parametrize("why", ["empty", "past max_len", "no queries"])
+@pytest.mark.parametrize("offsets", [False, True])
+def test_attention_without_a_key_in_sight(cuda, seqs, kv_heads, q_heads, why, offsets):
+    """Zero rows (left as they are where no sequence has them), the status
+    that says why, and a workspace that is ready for the next call."""
+    import torch
+
+    from aps2026_b200 import _lib, decode, ops
+
+    if why == "no queries" and not offsets:
+        pytest.skip("without offsets every sequence has a row")
+    g = _gen(seqs)
+    real = [1 + s % 5 for s in range(seqs)]
+    cache, table, _, _ = _filled(g, real, 8, kv_heads, 64)
+    q = _randn(g, seqs, q_heads, 64)
+    ws = decode.AttentionWorkspace(64, "cuda")
+    each = _i32(list(range(seqs + 1))) if offsets else None
+    lens, kw, status = _i32([0] * seqs), dict(max_len=8), 0
+    if why == "past max_len":
+        lens, kw, status = _i32(real), dict(max_len=0), _lib.B2_CHECK_KV4
+    out = torch.full_like(q, 5.0)
+    first = _i32([0] * (seqs + 1)) if why == "no queries" else each
+    for _ in range(2):
+        decode.attention_kv4_gpu(q, cache, table, _i32(real) if why == "no queries" else lens, out, q_offsets=first,
+                                 ws=ws, **kw)
+        assert ops.device_status() == status
+    assert bool((out == (5.0 if why == "no queries" else 0.0)).all())
+    want = torch.empty_like(q)
+    decode.attention_kv4_gpu(q, cache, table, _i32(real), want, q_offsets=each)
+    decode.attention_kv4_gpu(q, cache, table, _i32(real), out, q_offsets=each, ws=ws)
+    assert torch.equal(out, want) and bool((want != 0).any(-1).all()) and ops.device_status() == 0
+
+
+def test_attention_captured_at_zero_lengths(cuda):
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    seqs, g = 130, _gen(9)
+    real = [1 + s % 40 for s in range(seqs)]
+    cache, table, _, _ = _filled(g, real, 8, 4, 128)
+    q, lens = _randn(g, seqs, 16, 128), _i32([0] * seqs)
+    ws, out = decode.AttentionWorkspace(128, "cuda"), torch.full_like(q, 5.0)
+    run = lambda: decode.attention_kv4_gpu(q, cache, table, lens, out, ws=ws)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    graph.replay()
+    assert bool((out == 0).all())
+    lens.copy_(_i32(real))
+    graph.replay()
+    want = torch.empty_like(q)
+    decode.attention_kv4_gpu(q, cache, table, lens, want)
+    assert torch.equal(out, want) and bool((want != 0).any(-1).all())
+    lens.zero_()
+    graph.replay()
+    assert bool((out == 0).all()) and ops.device_status() == 0
