@@ -1431,7 +1431,8 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride, v
     a.counters = static_cast<unsigned*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.counters + kMaxGrid);
     a.part_o = a.part_ml + 2 * kMaxGrid * kRows * 2;
-    a.window = static_cast<unsigned>(window < 0x7FFFFFFFu ? window : 0);  // a window past every length: none
+    // a window past every length is none; a smaller one leaves positions minus windows inside an int
+    a.window = static_cast<unsigned>(window < max_len ? window : 0);
     a.sinks = static_cast<unsigned>(sinks < 0x7FFFFFFFu ? sinks : 0x7FFFFFFFu);
     cudaStream_t s = as_stream(stream);
     cudaError_t e;

@@ -73,3 +73,24 @@ def test_attention_captured_at_zero_lengths(cuda):
     lens.zero_()
     graph.replay()
     assert bool((out == 0).all()) and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 9, 2 ** 31, 2 ** 40, 20, 21])
+@pytest.mark.parametrize("q_heads", [1, 6])
+def test_attention_window_past_every_length(cuda, window, q_heads):
+    """The same as no window, with more query rows than positions too."""
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g = _gen(q_heads)
+    lens, queries = [3, 20], [8, 4]
+    cache, table, _, _ = _filled(g, lens, 8, 1, 64)
+    q = _randn(g, 12, q_heads, 64)
+    outs = []
+    for w in (0, window):
+        outs.append(torch.full_like(q, 5.0))
+        decode.attention_kv4_gpu(q, cache, table, _i32(lens), outs[-1], q_offsets=_i32([0, 8, 12]), max_queries=8,
+                                 max_len=20, window=w, sinks=1)
+    assert torch.equal(*outs) and ops.device_status() == 0
+    assert bool((outs[0][:5] == 0).all()) and bool((outs[0][5:] != 0).any(-1).all())
