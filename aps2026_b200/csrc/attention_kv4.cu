@@ -416,6 +416,15 @@ __device__ __forceinline__ void affine_operand(float q_sum, unsigned c, unsigned
 __device__ __forceinline__ float reference_for(float top, float q_scale, unsigned exponent) {
     return fmaf(top, q_scale, static_cast<float>(max(static_cast<int>(exponent) - 137, -71)));
 }
+// The same for one key, by its own steps: one that is not finite has no part in it.
+template <unsigned G>
+__device__ __forceinline__ float reference_for_key(float x, float q_scale, const unsigned* params) {
+    unsigned s = 0;
+#pragma unroll
+    for (unsigned g = 0; g < G; ++g)
+        if ((params[g] & 0x7F80u) != 0x7F80u) s = max(s, params[g] & 0x7F80u);
+    return reference_for(x, q_scale, s >> 7);
+}
 
 __device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, unsigned tok, int j, int pos) {
     return ((valid >> tok) & 1u) && j <= pos &&
@@ -530,8 +539,11 @@ struct Wide {
         }
 
         // ---- the reference: p s is to stay below 2^15 ----
-        // A thread packs p s of its own keys only, so each tests its own; what has
-        // to be exchanged is exchanged when some reference has to rise.
+        // A thread packs p s of its own keys only, so each tests its own, the top
+        // score against the largest step first. Only where that may be too much
+        // are keys taken one by one, each score with its own steps -- a large step
+        // of a key that the row does not see, or gives no weight, must not raise
+        // the reference: the others' p s would sink below fp16 -- and exchanged.
         float top = kNegInf;
         unsigned top_w = vp[0][0];  // maxima of both halves of the words: s is the lower
 #pragma unroll
@@ -543,14 +555,11 @@ struct Wide {
         }
         float need = reference_for(top, q_scale, top_w >> 7 & 0xFFu);
         if (__any_sync(0xffffffffu, need > ref + 4.0f)) {
-            if ((top_w & 0x7F80u) == 0x7F80u) {  // a step that is not finite has no part in the reference
-                unsigned finite_s = 0;
+            need = kNegInf;
 #pragma unroll
-                for (unsigned b = 0; b < 4; ++b)
-#pragma unroll
-                    for (unsigned i = 0; i < 2 * G; ++i)
-                        if ((vp[b][i] & 0x7F80u) != 0x7F80u) finite_s = max(finite_s, vp[b][i] & 0x7F80u);
-                need = reference_for(top, q_scale, finite_s >> 7);
+            for (unsigned b = 0; b < 4; ++b) {
+                const float2 y = f2_unpack(x[b]);
+                need = fmaxf(need, fmaxf(reference_for_key<G>(y.x, q_scale, vp[b]), reference_for_key<G>(y.y, q_scale, vp[b] + G)));
             }
             need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 1));
             need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 2));
@@ -769,9 +778,7 @@ struct Narrow {
             }
         }
 
-        // ---- the references: p s is to stay below 2^15 ----
-        // A thread packs p s of its own keys only, so each tests its own; what
-        // has to be exchanged is exchanged when some reference has to rise.
+        // ---- the references: p s is to stay below 2^15 (as in Wide) ----
         {
             const float2 x0 = f2_unpack(x[0]), x1 = f2_unpack(x[1]), scale = f2_unpack(q_scale), old = f2_unpack(ref);
             const float top0 = fmaxf(x0.x, x1.x), top1 = fmaxf(x0.y, x1.y);
@@ -780,16 +787,8 @@ struct Narrow {
             const unsigned exponent = top_w >> 7 & 0xFFu;
             float need0 = reference_for(top0, scale.x, exponent), need1 = reference_for(top1, scale.y, exponent);
             if (__any_sync(0xffffffffu, need0 > old.x + 4.0f || need1 > old.y + 4.0f)) {
-                if (exponent == 0xFFu) {  // a step that is not finite has no part in the reference
-                    unsigned finite_s = 0;
-#pragma unroll
-                    for (unsigned h = 0; h < 2; ++h)
-#pragma unroll
-                        for (unsigned g = 0; g < G; ++g)
-                            if ((vp[h][g] & 0x7F80u) != 0x7F80u) finite_s = max(finite_s, vp[h][g] & 0x7F80u);
-                    need0 = reference_for(top0, scale.x, finite_s >> 7);
-                    need1 = reference_for(top1, scale.y, finite_s >> 7);
-                }
+                need0 = fmaxf(reference_for_key<G>(x0.x, scale.x, vp[0]), reference_for_key<G>(x1.x, scale.x, vp[1]));
+                need1 = fmaxf(reference_for_key<G>(x0.y, scale.y, vp[0]), reference_for_key<G>(x1.y, scale.y, vp[1]));
 #pragma unroll
                 for (unsigned i = 2; i < 32; i *= 2) {
                     need0 = fmaxf(need0, __shfl_xor_sync(0xffffffffu, need0, i));

@@ -94,3 +94,61 @@ def test_attention_window_past_every_length(cuda, window, q_heads):
                                  max_len=20, window=w, sinks=1)
     assert torch.equal(*outs) and ops.device_status() == 0
     assert bool((outs[0][:5] == 0).all()) and bool((outs[0][5:] != 0).any(-1).all())
+
+
+def _append_at(cache, table, pos, k, v):
+    from aps2026_b200 import decode
+
+    decode.kv4_append_gpu(k, v, _i32([0]), _i32([pos]), cache, table)
+    decode.kv4_read_gpu(cache, table, _i32([0]), _i32([pos]), k, v)
+
+
+def _one_row64(q, k, v, scale):
+    import torch
+
+    kv_heads = k.shape[1]
+    w = torch.softmax(q.double().view(kv_heads, -1, q.shape[-1]) @ k.double().permute(1, 2, 0) * scale, -1)
+    return (w @ v.double().transpose(0, 1)).view(q.shape)
+
+
+# what the arithmetic below may cost a row: scores of some 2^3 held to 2^-20 of
+# their terms' sum move every weight by 2^-17 of itself
+ROW = 2.0 ** -17
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_heads", [2, 8])       # four rows of a KV head, and more
+@pytest.mark.parametrize("outlier", [2.0 ** 12, 2.0 ** 36, 2.0 ** 100])
+@pytest.mark.parametrize("where", ["behind the mask", "out of the window", "far below in score"])
+def test_attention_large_values_that_carry_no_weight(cuda, dim, q_heads, outlier, where):
+    """A value with a step many times the others', which a row does not see or
+    gives no weight, costs the row nothing."""
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g, n, kv_heads = _gen(dim + q_heads), 75, 1
+    cache, table, k, v = _filled(g, [n], 16, kv_heads, dim)
+    q = _randn(g, 2, q_heads, dim)
+    window, at = (0, n - 1) if where != "out of the window" else (40, n - 41)
+    far_k = k[at:at + 1].clone()
+    if where == "far below in score":
+        # against every query row's sum
+        at, far_k = n - 2, torch.full_like(far_k, 0.0)
+        q = q.abs()
+        far_k -= 200.0
+    far_v = _randn(g, 1, kv_heads, dim) * outlier
+    _append_at(cache, table, at, far_k, far_v)
+    out = torch.empty_like(q)
+    decode.attention_kv4_gpu(q, cache, table, _i32([n]), out, q_offsets=_i32([0, 2]), max_queries=2, window=window)
+    if where == "behind the mask":        # of the first row
+        rows, seen = [0], [slice(0, n - 1)]
+    elif where == "out of the window":    # of the last row
+        rows, seen = [1], [slice(n - 40, n)]
+    else:
+        keep = [j for j in range(n) if j != at]
+        rows, seen = [0, 1], [[j for j in keep if j < n - 1], keep]
+    for row, s in zip(rows, seen):
+        want = _one_row64(q[row], k[s], v[s], dim ** -0.5)
+        assert float((out[row].double() - want).norm() / want.norm()) < ROW
+    assert ops.device_status() == 0
