@@ -416,14 +416,27 @@ __device__ __forceinline__ void affine_operand(float q_sum, unsigned c, unsigned
 __device__ __forceinline__ float reference_for(float top, float q_scale, unsigned exponent) {
     return fmaf(top, q_scale, static_cast<float>(max(static_cast<int>(exponent) - 137, -71)));
 }
-// The same for one key, by its own steps: one that is not finite has no part in it.
+// The same for one key, by its own parameters. A minimum counts as a step 2^80
+// below it, which keeps sums of p m over 2^28 keys in fp32 where steps are tiny
+// or zero; what is not finite has no part in it.
 template <unsigned G>
 __device__ __forceinline__ float reference_for_key(float x, float q_scale, const unsigned* params) {
-    unsigned s = 0;
+    int exponent = 0;
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g)
-        if ((params[g] & 0x7F80u) != 0x7F80u) s = max(s, params[g] & 0x7F80u);
-    return reference_for(x, q_scale, s >> 7);
+    for (unsigned g = 0; g < G; ++g) {
+        const int s = params[g] >> 7 & 0xFFu, m = params[g] >> 23 & 0xFFu;
+        if (s != 0xFF) exponent = max(exponent, s);
+        if (m != 0xFF) exponent = max(exponent, m - 80);
+    }
+    return reference_for(x, q_scale, static_cast<unsigned>(exponent));
+}
+// Minima from here on may need that; below it p m is in range whatever the
+// steps are (p < 2^75 at the least step reference_for counts).
+constexpr float kLargeMinimum = 1048576.0f;
+// max(top, |m|) of a parameter word: m is the word's high half, so the word is
+// m but for its last bits.
+__device__ __forceinline__ float max_minimum(float top, unsigned params) {
+    return fmaxf(top, fabsf(__uint_as_float(params)));
 }
 
 __device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, unsigned tok, int j, int pos) {
@@ -544,17 +557,20 @@ struct Wide {
         // are keys taken one by one, each score with its own steps -- a large step
         // of a key that the row does not see, or gives no weight, must not raise
         // the reference: the others' p s would sink below fp16 -- and exchanged.
-        float top = kNegInf;
+        float top = kNegInf, top_m = 0.0f;
         unsigned top_w = vp[0][0];  // maxima of both halves of the words: s is the lower
 #pragma unroll
         for (unsigned b = 0; b < 4; ++b) {
             const float2 y = f2_unpack(x[b]);
             top = fmaxf(top, fmaxf(y.x, y.y));
 #pragma unroll
-            for (unsigned i = 0; i < 2 * G; ++i) top_w = __vmaxu2(top_w, vp[b][i]);
+            for (unsigned i = 0; i < 2 * G; ++i) {
+                top_w = __vmaxu2(top_w, vp[b][i]);
+                top_m = max_minimum(top_m, vp[b][i]);
+            }
         }
         float need = reference_for(top, q_scale, top_w >> 7 & 0xFFu);
-        if (__any_sync(0xffffffffu, need > ref + 4.0f)) {
+        if (__any_sync(0xffffffffu, need > ref + 4.0f || top_m >= kLargeMinimum)) {
             need = kNegInf;
 #pragma unroll
             for (unsigned b = 0; b < 4; ++b) {
@@ -785,8 +801,10 @@ struct Narrow {
             unsigned top_w = __vmaxu2(vp[0][0], vp[1][0]);  // maxima of both halves: s is the lower
             if (G == 2) top_w = __vmaxu2(top_w, __vmaxu2(vp[0][G - 1], vp[1][G - 1]));
             const unsigned exponent = top_w >> 7 & 0xFFu;
+            float top_m = max_minimum(max_minimum(0.0f, vp[0][0]), vp[1][0]);
+            if (G == 2) top_m = max_minimum(max_minimum(top_m, vp[0][G - 1]), vp[1][G - 1]);
             float need0 = reference_for(top0, scale.x, exponent), need1 = reference_for(top1, scale.y, exponent);
-            if (__any_sync(0xffffffffu, need0 > old.x + 4.0f || need1 > old.y + 4.0f)) {
+            if (__any_sync(0xffffffffu, need0 > old.x + 4.0f || need1 > old.y + 4.0f || top_m >= kLargeMinimum)) {
                 need0 = fmaxf(reference_for_key<G>(x0.x, scale.x, vp[0]), reference_for_key<G>(x1.x, scale.x, vp[1]));
                 need1 = fmaxf(reference_for_key<G>(x0.y, scale.y, vp[0]), reference_for_key<G>(x1.y, scale.y, vp[1]));
 #pragma unroll

@@ -152,3 +152,29 @@ def test_attention_large_values_that_carry_no_weight(cuda, dim, q_heads, outlier
         want = _one_row64(q[row], k[s], v[s], dim ** -0.5)
         assert float((out[row].double() - want).norm() / want.norm()) < ROW
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_heads", [2, 8])
+@pytest.mark.parametrize("value", [1e10, -1e16, 3e25, -2.0 ** 100])
+@pytest.mark.parametrize("first_group_alone", [False, True])
+def test_attention_constant_values(cuda, dim, q_heads, value, first_group_alone):
+    """Groups of one value have steps of zero; their weighted sum is that value."""
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g, n = _gen(dim), 333
+    cache, table, k, v = _filled(g, [n], 16, 1, dim)
+    value = float(torch.tensor(value).bfloat16())  # held as it is
+    v[..., :64 if first_group_alone else dim] = value
+    seq, pos = _i32([0] * n), torch.arange(n, device="cuda", dtype=torch.int32)
+    decode.kv4_append_gpu(k, v, seq, pos, cache, table)
+    decode.kv4_read_gpu(cache, table, seq, pos, k, v)
+    q, out = _randn(g, 1, q_heads, dim), torch.empty(1, q_heads, dim, device="cuda")
+    decode.attention_kv4_gpu(q, cache, table, _i32([n]), out)
+    want = _one_row64(q, k, v, dim ** -0.5)
+    for part in range(0, dim, 64):
+        a, b = out[..., part:part + 64].double(), want[..., part:part + 64]
+        assert float((a - b).norm() / b.norm()) < (ROW if abs(value) < 2.0 ** 90 or part == 0 else 2.0 ** -12)
+    assert ops.device_status() == 0
