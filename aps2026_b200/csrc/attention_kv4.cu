@@ -67,7 +67,7 @@ struct AttnKv4Args {
     const std::uint32_t* lens;
     unsigned max_queries, max_len;
     unsigned tiles;                     // row tiles per sequence: ceil(max_queries * group / ROWS)
-    float scale_log2, q_sign;           // |scale| * log2(e); the scale's sign, 0 for scale 0
+    float scale, q_sign;                // |scale| (1 for scale 0); the scale's sign, 0 for scale 0
     unsigned window, sinks;
     unsigned* counters;                 // [kMaxGrid], zero between calls
     float* part_ml;                     // [2 kMaxGrid][8][2]: reference, sum
@@ -956,24 +956,21 @@ __device__ __forceinline__ void place_query(const AttnKv4Args& a, const float (&
     if (warp >= Rows::ROWS) return;
     float top = 0.0f, sum[G];
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) sum[g] = 0.0f;
-#pragma unroll
-    for (unsigned e = 0; e < D / 32; ++e) {
-        top = fmaxf(top, fabsf(v[e]));
-        sum[e / 2] += v[e];
-    }
+    for (unsigned e = 0; e < D / 32; ++e) top = fmaxf(top, fabsf(v[e]));
     top = warp_max(top);
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) sum[g] = warp_sum(sum[g]);
     // 2^e with top * 2^e in [2^9, 2^10)
     int e = 136 - static_cast<int>(__float_as_uint(top) >> 23);
     e = top == 0.0f ? 0 : max(-118, min(e, 100));
     const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
-    if (lane == 0) {
-        // positive, so that a masked score stays -inf
-        sm.q_scale[warp] = fmaxf(a.scale_log2 * __uint_as_float(static_cast<unsigned>(127 - e) << 23), 1.17549435e-38f);
+    // sums of scaled queries, and the scale back before log2(e): neither passes an end of fp32 on the way
 #pragma unroll
-        for (unsigned g = 0; g < G; ++g) sm.q_sum[warp][g] = sum[g] * up;
+    for (unsigned g = 0; g < G; ++g) sum[g] = warp_sum(v[2 * g] * up + v[2 * g + 1] * up);
+    if (lane == 0) {
+        const float down = a.scale * __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+        // positive, so that a masked score stays -inf
+        sm.q_scale[warp] = fmaxf(down * 1.4426950408889634f, 1.17549435e-38f);
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) sm.q_sum[warp][g] = sum[g];
     }
     // dimension d = w * 32 + c * 8 + i: nibble i of word w of lane (row, c)
 #pragma unroll
@@ -1435,7 +1432,7 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride, v
     a.q_offsets = q_offsets; a.lens = lens;
     a.max_queries = static_cast<unsigned>(max_queries); a.max_len = static_cast<unsigned>(max_len);
     if (!(std::fabs(scale) < INFINITY)) return invalid("b2_attention_kv4: scale must be finite");
-    a.scale_log2 = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.4426950408889634f;
+    a.scale = scale == 0.0f ? 1.0f : std::fabs(scale);
     a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
     // up to four rows of a KV head per sequence: the four-row form
     const bool narrow = max_queries * a.group <= 4;

@@ -178,3 +178,21 @@ def test_attention_constant_values(cuda, dim, q_heads, value, first_group_alone)
         a, b = out[..., part:part + 64].double(), want[..., part:part + 64]
         assert float((a - b).norm() / b.norm()) < (ROW if abs(value) < 2.0 ** 90 or part == 0 else 2.0 ** -12)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_heads", [2, 8])
+@pytest.mark.parametrize("k", [-100, 126])
+def test_attention_queries_of_one_sign_and_any_size(cuda, q_heads, k):
+    """Queries times 2^k at a scale of 2^-k are the same queries, bit for bit,
+    also where their sum passes fp32's end, or the scale its start in base 2."""
+    import torch
+
+    from aps2026_b200 import decode
+
+    g, n = _gen(q_heads + 8), 333
+    cache, table, _, _ = _filled(g, [n], 16, 2, 128)
+    q, want = torch.rand((1, q_heads, 128), generator=g, device="cuda") + 0.9, torch.empty(1, q_heads, 128, device="cuda")
+    out = torch.empty_like(want)
+    decode.attention_kv4_gpu(q, cache, table, _i32([n]), want, scale=0.0625)
+    decode.attention_kv4_gpu(q * 2.0 ** k, cache, table, _i32([n]), out, scale=0.0625 * 2.0 ** -k)
+    assert bool(want.isfinite().all()) and torch.equal(out, want)
