@@ -97,6 +97,12 @@ const At& whole(const At& t, std::initializer_list<std::int64_t> shape, at::Scal
                       " tensor on CUDA device " + std::to_string(device)};
     return t;
 }
+// Refuses a buffer that is not `bytes` adjacent bytes at least.
+void bytes_of(const At& t, std::size_t bytes, const char* what) {
+    if (!t.is_contiguous() || t.nbytes() < bytes)
+        throw Refusal{std::string(what) + ": expected " + std::to_string(bytes) + " contiguous bytes, got " +
+                      (t.is_contiguous() ? std::to_string(t.nbytes()) : "a tensor that is not contiguous")};
+}
 
 // Five arguments of a KVCache4 (data, pages, page_size, kv_heads, head_dim) and its page table.
 b2_kv4_cache cache_of(PyObject* const* a, PyObject* page_table, bool writes, int* device) {
@@ -114,6 +120,10 @@ b2_kv4_cache cache_of(PyObject* const* a, PyObject* page_table, bool writes, int
     c.page_table = static_cast<const std::uint32_t*>(table.const_data_ptr());
     c.seqs = static_cast<std::size_t>(table.size(0));
     c.max_pages = static_cast<std::size_t>(table.size(1));
+    // the kernels bound pages by c.pages alone (a description that has no page size is refused by the call itself)
+    std::size_t page = 0;
+    if (b2_kv4_page_bytes(c.page_size, c.kv_heads, c.head_dim, &page) == B2_OK)
+        bytes_of(data, page && c.pages > SIZE_MAX / page ? SIZE_MAX : c.pages * page, "cache");
     return c;
 }
 
@@ -230,6 +240,7 @@ PyObject* attention_kv4(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           ws_bytes = size(a[16], "attention_kv4: workspace bytes");
         const float scale = a[12] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : number(a[12]);
         if (ws.get_device() != device) throw Refusal{"attention_kv4: the workspace is on another device"};
+        bytes_of(ws, ws_bytes, "attention_kv4 workspace");
         void* workspace = ws.mutable_data_ptr();
         return unlocked([&] {
             return b2_attention_kv4(qh.data, qh.by_row, qh.by_head, out, dtype, static_cast<std::size_t>(rows),
@@ -264,6 +275,7 @@ PyObject* moe_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const float quantum = number(a[5]), tie_eps = number(a[6]);
         const std::uint32_t gates = static_cast<std::uint32_t>(size(a[7], "moe_decode: gates"));
         const std::size_t ws_bytes = size(a[9], "moe_decode: workspace bytes");
+        bytes_of(ws, ws_bytes, "moe_decode workspace");
         const std::size_t ld_x = static_cast<std::size_t>(T > 1 ? x.stride(0) : H),
                           ld_out = static_cast<std::size_t>(T > 1 ? out.stride(0) : H);
         void *to = out.mutable_data_ptr(), *workspace = ws.mutable_data_ptr();

@@ -196,3 +196,25 @@ def test_attention_queries_of_one_sign_and_any_size(cuda, q_heads, k):
     decode.attention_kv4_gpu(q, cache, table, _i32([n]), want, scale=0.0625)
     decode.attention_kv4_gpu(q * 2.0 ** k, cache, table, _i32([n]), out, scale=0.0625 * 2.0 ** -k)
     assert bool(want.isfinite().all()) and torch.equal(out, want)
+
+
+def test_workspaces_smaller_than_they_say_are_refused(cuda):
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g = _gen(3)
+    cache, table, _, _ = _filled(g, [5], 8, 1, 64)
+    q, x = _randn(g, 1, 4, 64), _randn(g, 2, 64)
+    gate_up, down, logits = _randn(g, 4, 32, 64), _randn(g, 4, 64, 16), _randn(g, 2, 4)
+    for cut in (slice(16), slice(0, None, 2)):
+        attention, moe = decode.AttentionWorkspace(64, "cuda"), decode.MoeWorkspace(2, 16, "cuda")
+        attention.buf, moe.buf = attention.buf[cut], moe.buf[cut]
+        with pytest.raises(ops.InvalidArgument, match="workspace: expected"):
+            decode.attention_kv4_gpu(q, cache, table, _i32([5]), torch.empty_like(q), ws=attention)
+        with pytest.raises(ops.InvalidArgument, match="workspace: expected"):
+            decode.moe_decode_gpu(x, logits, gate_up, down, torch.empty_like(x), ws=moe)
+    cache.pages += 1
+    with pytest.raises(ops.InvalidArgument, match="cache: expected"):
+        decode.attention_kv4_gpu(q, cache, table, _i32([5]), torch.empty_like(q))
+    assert ops.device_status() == 0
