@@ -548,6 +548,70 @@ struct Ring {
     }
 };
 
+// ---- infinities ---------------------------------------------------------------------------
+//
+// In parts an infinite operand is inf - inf, and so is a finite one whose high
+// part rounds up to infinity; a part that is 0 makes an infinite weight a NaN.
+// All of that ends in a NaN sum, so a sum that is NaN is taken once more
+// without parts: it comes out infinite, or finite, where a plain fp32 sum does.
+// Only that case costs time (a token of NaN: its rows' sums up to the first NaN).
+__device__ __forceinline__ float wide(float v) { return v; }
+__device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename X, typename W>
+__device__ float plain_dot(const X* x, const W* w, unsigned n) {
+    float sum = 0.0f;
+    for (unsigned k = 0; k < n && sum == sum; ++k) sum = fmaf(wide(w[k]), wide(x[k]), sum);
+    return sum;
+}
+// An activation from here on, or NaN, is unusual: the largest bf16, up to which
+// rounding makes no part infinite.
+constexpr float kUnusual = 3.3895313892515355e38f;
+// Stores activation v, which is unusual, in its parts: taken again where it is
+// NaN; its high parts truncated, and an infinite one alone.
+template <typename X, typename W>
+__device__ __noinline__ void put_unusual(float v, const X* x, const W* gate_row, std::size_t to_up, unsigned H, void* act,
+                                         std::size_t at, std::size_t plane) {
+    if (v != v && sizeof(X) + sizeof(W) > 4) {  // else nothing was in parts
+        const float gate = plain_dot(x, gate_row, H), up = plain_dot(x, gate_row + to_up, H);
+        v = gate / (1.0f + expf(-gate)) * up;
+    }
+    constexpr unsigned PARTS = kParts<float, W>;
+    for (unsigned q = 0; q < PARTS; ++q) {
+        const float b = sizeof(W) == 2 ? wide(__float2bfloat16_rz(v))
+                                       : v != v ? v : __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
+        if constexpr (sizeof(W) == 2) static_cast<__nv_bfloat16*>(act)[q * plane + at] = __float2bfloat16_rz(v);
+        else static_cast<float*>(act)[q * plane + at] = b;
+        v = isinf(v) ? 0.0f : v - b;
+    }
+}
+// sum_k w[k] act[k], activations in their planes.
+template <typename W>
+__device__ float plain_dot_planes(const void* act, std::size_t at, std::size_t plane, const W* w, unsigned n) {
+    float sum = 0.0f;
+    for (unsigned k = 0; k < n && sum == sum; ++k) {
+        float v;
+        if constexpr (sizeof(W) == 2) {
+            const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(act) + at + k;
+            v = wide(a[0]) + wide(a[plane]) + wide(a[2 * plane]);
+        } else {
+            const float* a = static_cast<const float*>(act) + at + k;
+            v = a[0] + a[plane];
+        }
+        sum = fmaf(wide(w[k]), v, sum);
+    }
+    return sum;
+}
+// A token's output that is NaN, taken again: y0, y1 its experts' sums, `at`
+// its first expert's activations, w0 and w1 its rows of w_down.
+template <typename W>
+__device__ __noinline__ float output_again(float y0, float y1, float g0, float g1, const void* act, std::size_t at,
+                                           std::size_t act_ld, std::size_t plane, const W* w0, const W* w1, unsigned n) {
+    if (y0 != y0) y0 = plain_dot_planes(act, at, plane, w0, n);
+    if (y1 != y1) y1 = plain_dot_planes(act, at + act_ld, plane, w1, n);
+    return g0 * y0 + g1 * y1;
+}
+
 // ---- launch 1 ---------------------------------------------------------------------------
 
 // Item j: group j / tiles, rows j % tiles * 8 MT ... of its gate and up.
@@ -710,7 +774,11 @@ moe_gate_up(MoeDecodeArgs a, unsigned tiles) {
             const std::size_t at = static_cast<std::size_t>(to) * a.act_ld + i0 + row;
             const std::size_t plane = static_cast<std::size_t>(2) * a.T * a.act_ld;
             float v = i0 + row < a.I ? gate / (1.0f + expf(-gate)) * up : 0.0f;
-            if constexpr (sizeof(W) == 2) {
+            if (!(fabsf(v) < kUnusual)) {
+                put_unusual(v, static_cast<const X*>(a.x) + to / 2 * a.ld_x,
+                            static_cast<const W*>(a.w_gate_up) + (static_cast<std::size_t>(e) * 2 * a.I + i0 + row) * a.H,
+                            static_cast<std::size_t>(a.I) * a.H, a.H, a.act, at, plane);
+            } else if constexpr (sizeof(W) == 2) {
                 __nv_bfloat16* act = static_cast<__nv_bfloat16*>(a.act);
 #pragma unroll
                 for (unsigned q = 0; q < 3; ++q) {
@@ -881,7 +949,14 @@ moe_down(MoeDecodeArgs a, unsigned per) {
             y[0] += sm.sums[p * 2 * T + 2 * t][h];
             y[1] += sm.sums[p * 2 * T + 2 * t + 1][h];
         }
-        const float v = sm.plan.gate[2 * t] * y[0] + sm.plan.gate[2 * t + 1] * y[1];
+        const float g0 = sm.plan.gate[2 * t], g1 = sm.plan.gate[2 * t + 1];
+        float v = g0 * y[0] + g1 * y[1];
+        if (v != v) {
+            const W* rows = static_cast<const W*>(a.w_down) + static_cast<std::size_t>(h0 + h) * a.I;
+            const std::size_t of_expert = static_cast<std::size_t>(a.H) * a.I;
+            v = output_again(y[0], y[1], g0, g1, a.act, static_cast<std::size_t>(2 * (t0 + t)) * a.act_ld, a.act_ld, plane,
+                             rows + (sm.plan.pair[t] & 0xFFu) * of_expert, rows + (sm.plan.pair[t] >> 8) * of_expert, a.I);
+        }
         X* out = static_cast<X*>(a.out) + (t0 + t) * a.ld_out + h0 + h;
         if constexpr (sizeof(X) == 2) *out = __float2bfloat16_rn(v);
         else *out = v;

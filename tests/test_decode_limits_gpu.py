@@ -218,3 +218,70 @@ def test_workspaces_smaller_than_they_say_are_refused(cuda):
     with pytest.raises(ops.InvalidArgument, match="cache: expected"):
         decode.attention_kv4_gpu(q, cache, table, _i32([5]), torch.empty_like(q))
     assert ops.device_status() == 0
+
+
+def _experts_plain(x, logits, gate_up, down):
+    """The expert layer in 64 bits, but infinite where its activations or its
+    result are so in the operator's types."""
+    import torch
+
+    from aps2026_b200 import ops
+
+    pairs = ops.moe_route_gpu(logits).routes.long().sort(1).values
+    inter, rows, mag = down.shape[2], [], []
+    for t, pair in enumerate(pairs.tolist()):
+        y, m = 0.0, 0.0
+        for e in pair:
+            gate, up = (gate_up[e].double() @ x[t].double()).split(inter)
+            a = (gate / (1 + torch.exp(-gate)) * up).float().double()
+            y, m = y + 0.5 * (down[e].double() @ a), m + 0.5 * (down[e].double().abs() @ a.abs())
+        rows.append(y)
+        mag.append(m)
+    out = torch.stack(rows)
+    held = out.to(x.dtype).double()
+    return torch.where(held.isfinite(), out, held), torch.stack(mag)
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("H,I", [(64, 24), (65, 27), (3000, 40)])
+@pytest.mark.parametrize("xt,wt", [("float32", "bfloat16"), ("bfloat16", "bfloat16"), ("float32", "float32"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("what", ["x infinite", "x at the end", "gate weight infinite", "down weight infinite", "activation overflows"])
+def test_experts_keep_infinities_and_the_largest_numbers(cuda, T, H, I, xt, wt, what):
+    """Infinite where a plain sum is, of its sign, and finite where that is."""
+    import torch
+
+    from aps2026_b200 import decode
+
+    g, E = _gen(T + H), 4
+    xt, wt = getattr(torch, xt), getattr(torch, wt)
+    x, logits = _randn(g, T, H), _randn(g, T, E)
+    gate_up, down = _randn(g, E, 2 * I, H) / math.sqrt(H), _randn(g, E, H, I) / math.sqrt(I)
+    sign = torch.where(torch.arange(H, device="cuda") % 3 == 0, -1.0, 1.0)[:, None]
+    if what == "x infinite":
+        x[1, H // 2] = float("inf")
+        gate_up, down = gate_up.abs(), down.abs() * sign
+    elif what == "x at the end":
+        x[1] = x[1].sign() * 3.4e38
+        gate_up = gate_up * 2.0 ** -100
+    elif what == "gate weight infinite":
+        gate_up[2, I // 2, H // 2] = float("inf")
+        down = down.abs() * sign
+    elif what == "down weight infinite":
+        down[2, H // 2, I // 2] = float("inf")
+    else:
+        x[1] = x[1].abs() * 1e20
+        gate_up, down = gate_up.abs(), down.abs() * sign
+    x = x.to(xt) if what != "x at the end" else torch.where(x.to(xt).isinf(), 3.3e38 * x.sign(), x).to(xt)
+    gate_up, down = gate_up.to(wt), down.to(wt)
+    out = torch.full_like(x, 5.0)
+    decode.moe_decode_gpu(x, logits, gate_up, down, out)
+    want, mag = _experts_plain(x, logits, gate_up, down)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.isinf(), want.isinf()) and torch.equal(out[out.isinf()].double(), want[want.isinf()])
+    if what in ("x infinite", "activation overflows"):
+        assert bool(out[1].isinf().all())
+    # sums of inputs held to 16 bits or more, a row at a time
+    fine = want.isfinite()
+    scale = torch.where(fine, mag, 0.0).mean(1, keepdim=True)
+    bound = 2.0 ** -14 * (mag + scale) + (2.0 ** -8 * want.abs() if xt == torch.bfloat16 else 0)
+    assert bool(((out.double() - want).abs() <= bound)[fine].all())
