@@ -28,3 +28,36 @@ def test_a_cache_smaller_than_it_says_is_refused(change):
                  lambda: decode.attention_kv4_gpu(k, cache, _table(), i, k, ws=ws)):
         with pytest.raises(ops.InvalidArgument, match="cache: expected"):
             call()
+
+
+# Experts with fp32 activations, error of the output relative to its size: a
+# product is off by 2^-22 of itself three times at most (either operand's last
+# part, the product of the low parts), apart from each other in sign; the
+# gate, the up and the down product add up to three such sums.
+EXPERTS = 2.0 ** -19
+
+
+def _experts(x, gate_up, down, cut=lambda t: t):
+    """One expert in 64 bits; cut: what its activations are held as."""
+    import torch
+
+    gate, up = (cut(x) @ gate_up.t()).chunk(2, 1)
+    return cut(gate * torch.sigmoid(gate) * up) @ down.t()
+
+
+@pytest.mark.parametrize("H,I", [(256, 40), (4096, 448), (1001, 333)])
+def test_the_experts_bound_tells_16_bits_from_24(H, I):
+    """What the bound is for: operands held to 24 bits pass it, to 16 or 17 do not."""
+    import torch
+
+    def held_to(bits):
+        drop = 53 - bits
+        return lambda t: (t.contiguous().view(torch.int64) >> drop << drop).view(torch.float64)
+
+    g = torch.Generator().manual_seed(H)
+    rand = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)  # noqa: E731
+    x, gate_up, down = rand(9, H), rand(2 * I, H) / H ** 0.5, rand(H, I) / I ** 0.5
+    want = _experts(x, gate_up, down)
+    off = lambda bits: float((_experts(x, gate_up, down, held_to(bits)) - want).norm() / want.norm())  # noqa: E731
+    assert off(24) < EXPERTS and off(22) < EXPERTS
+    assert off(17) > EXPERTS and off(16) > EXPERTS
