@@ -26,7 +26,7 @@
 #include <string>
 
 #include "fastexp.cuh"
-#include "route_pick.cuh"
+#include "quantize.cuh"
 #include "rowload.cuh"
 
 namespace b2 {
@@ -60,13 +60,50 @@ struct RouteArgs {
     std::size_t tiles;
 };
 
-// The two experts of token t (route_pick.cuh), also stored to routes[t].
+// The two experts of token t, first | second << 8, as k_moe_top2 picks
+// them (src/tensor.cu:1299-1328): the first scan takes an expert when its
+// quantized score beats the best so far by more than tie_eps, the second
+// scan does the same skipping the first pick; also stored to routes[t].
 __device__ __forceinline__ unsigned pick_top2(const RouteArgs& a, std::size_t t) {
     const unsigned E = static_cast<unsigned>(a.E);
     float sc[kMaxExperts];
-    load_scores(a.logits + t * a.E, E, sc);
-    const unsigned pair = top2_of_scores(sc, E, a.quantum, a.tie_eps);
-    reinterpret_cast<unsigned short*>(a.routes)[t] = static_cast<unsigned short>(pair);
+    const float* row = a.logits + t * a.E;
+    if ((E & 3u) == 0 && aligned16(row)) {
+#pragma unroll
+        for (unsigned e = 0; e < kMaxExperts; e += 4)
+            if (e < E) {
+                const float4 v = ld_stream(reinterpret_cast<const float4*>(row + e));
+                sc[e] = v.x; sc[e + 1] = v.y; sc[e + 2] = v.z; sc[e + 3] = v.w;
+            }
+    } else {
+#pragma unroll
+        for (unsigned e = 0; e < kMaxExperts; ++e)
+            if (e < E) sc[e] = __ldg(row + e);
+    }
+    int first = -1;
+    float first_value = -3.402823466e+38F;
+#pragma unroll
+    for (unsigned e = 0; e < kMaxExperts; ++e)
+        if (e < E) {
+            sc[e] = quantize(sc[e], a.quantum);
+            if (first < 0 || sc[e] > __fadd_rn(first_value, a.tie_eps)) {
+                first = static_cast<int>(e);
+                first_value = sc[e];
+            }
+        }
+    int second = -1;
+    float second_value = -3.402823466e+38F;
+#pragma unroll
+    for (unsigned e = 0; e < kMaxExperts; ++e)
+        if (e < E && static_cast<int>(e) != first) {
+            if (second < 0 || sc[e] > __fadd_rn(second_value, a.tie_eps)) {
+                second = static_cast<int>(e);
+                second_value = sc[e];
+            }
+        }
+    const unsigned short pair =
+        static_cast<unsigned short>(first) | (static_cast<unsigned short>(second) << 8);
+    reinterpret_cast<unsigned short*>(a.routes)[t] = pair;
     return pair;
 }
 

@@ -42,7 +42,7 @@
 
 #include <cuda_bf16.h>
 
-#include "route_pick.cuh"
+#include "quantize.cuh"
 
 namespace b2 {
 namespace {

@@ -285,3 +285,28 @@ def test_experts_keep_infinities_and_the_largest_numbers(cuda, T, H, I, xt, wt, 
     scale = torch.where(fine, mag, 0.0).mean(1, keepdim=True)
     bound = 2.0 ** -14 * (mag + scale) + (2.0 ** -8 * want.abs() if xt == torch.bfloat16 else 0)
     assert bool(((out.double() - want).abs() <= bound)[fine].all())
+
+
+@pytest.mark.parametrize("E", [2, 3, 15, 16, 17, 31, 32])
+@pytest.mark.parametrize("spread", [0.0, 0.004, 0.03, 1.0])
+def test_experts_are_those_of_the_routing(cuda, E, spread):
+    """Two implementations of one rule: around the margin and on the grid's
+    boundaries, with infinities and NaN among the scores."""
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g, T = _gen(E), 128
+    # expert e writes coordinate e
+    x, gate_up = torch.ones(T, 32, device="cuda"), torch.ones(E, 2, 32, device="cuda")
+    down = torch.eye(32, device="cuda")[:E, :, None].contiguous()
+    for odd in (None, float("nan"), float("inf"), -float("inf")):
+        logits = _randn(g, T, E) * spread
+        logits[::2] = (logits[::2] / 5e-4).round() * 5e-4      # grid points and the middles between them
+        logits[1::4] = (logits[1::4] / 2e-2).round() * 2e-2    # margins
+        if odd is not None:
+            logits[torch.rand(T, E, generator=g, device="cuda") < 0.2] = odd
+        out = torch.empty(T, 32, device="cuda")
+        decode.moe_decode_gpu(x, logits, gate_up, down, out)
+        want = torch.zeros(T, 32, device="cuda").scatter_(1, ops.moe_route_gpu(logits).routes.long(), 1.0)
+        assert torch.equal((out != 0).float(), want)
