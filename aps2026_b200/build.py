@@ -5,8 +5,9 @@ arch=compute_100a,code=sm_100a -lineinfo -O3``, IEEE division and square
 root, no fast-math: the routing quantiser and the LayerNorm need them), the
 host C++ by g++, and everything is linked into one shared library next to
 this file; pyext/ becomes _decode_calls.so, the Python calls of the decode step
-(g++ against torch's headers, linked to the library). Objects go to ``aps2026_b200/_build`` and are rebuilt only when a
-source or header is newer.
+(g++ against torch's headers, linked to the library). Objects go to
+``aps2026_b200/_build`` and are rebuilt only when a source or header is newer,
+the Python calls also when torch or Python is another.
 
 Run as ``python -m aps2026_b200.build [-v]`` (``-v`` prints ptxas register /
 spill / shared-memory use per kernel).
@@ -17,6 +18,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+from importlib import metadata
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -64,7 +66,9 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def _build_pyext() -> None:
     newest = max([PYEXT.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
-    if PYEXT_LIB.exists() and PYEXT_LIB.stat().st_mtime >= newest:
+    built_for = f"torch {metadata.version('torch')}, {sys.implementation.cache_tag}"
+    key = BUILD / "decode_calls.key"  # what the module there was built for
+    if (PYEXT_LIB.exists() and PYEXT_LIB.stat().st_mtime >= newest and key.exists() and key.read_text() == built_for):
         return
     import sysconfig
 
@@ -79,6 +83,7 @@ def _build_pyext() -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    key.write_text(built_for)
 
 
 def build(verbose: bool = False) -> Path:

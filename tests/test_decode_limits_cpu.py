@@ -61,3 +61,33 @@ def test_the_experts_bound_tells_16_bits_from_24(H, I):
     off = lambda bits: float((_experts(x, gate_up, down, held_to(bits)) - want).norm() / want.norm())  # noqa: E731
     assert off(24) < EXPERTS and off(22) < EXPERTS
     assert off(17) > EXPERTS and off(16) > EXPERTS
+
+
+@pytest.fixture
+def pyext_builds(monkeypatch, tmp_path):
+    """The extension module's builds, made by a compiler that only writes its output."""
+    from aps2026_b200 import build
+
+    runs = []
+
+    def compile_(cmd, **_):
+        runs.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return type("Result", (), dict(returncode=0, stdout="", stderr=""))
+
+    monkeypatch.setattr(build, "PYEXT_LIB", tmp_path / "_decode_calls.so")
+    monkeypatch.setattr(build, "BUILD", tmp_path)
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    return runs
+
+
+def test_the_extension_is_built_anew_for_another_torch(pyext_builds, monkeypatch):
+    from aps2026_b200 import build
+
+    build._build_pyext()
+    build._build_pyext()
+    assert len(pyext_builds) == 1
+    monkeypatch.setattr(build.metadata, "version", lambda name: "0.0.1")
+    build._build_pyext()
+    build._build_pyext()
+    assert len(pyext_builds) == 2
