@@ -7,7 +7,8 @@ host C++ by g++, and everything is linked into one shared library next to
 this file; pyext/ becomes _decode_calls.so, the Python calls of the decode step
 (g++ against torch's headers, linked to the library). Objects go to
 ``aps2026_b200/_build`` and are rebuilt only when a source or header is newer,
-the Python calls also when torch or Python is another.
+the Python calls also when torch or Python is another; without torch there
+are none, and the library is built alone.
 
 Run as ``python -m aps2026_b200.build [-v]`` (``-v`` prints ptxas register /
 spill / shared-memory use per kernel).
@@ -66,7 +67,11 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def _build_pyext() -> None:
     newest = max([PYEXT.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
-    built_for = f"torch {metadata.version('torch')}, {sys.implementation.cache_tag}"
+    try:
+        built_for = f"torch {metadata.version('torch')}, {sys.implementation.cache_tag}"
+    except metadata.PackageNotFoundError:
+        sys.stderr.write("torch is not installed: the library alone is built, without the decode step's Python calls\n")
+        return
     key = BUILD / "decode_calls.key"  # what the module there was built for
     if (PYEXT_LIB.exists() and PYEXT_LIB.stat().st_mtime >= newest and key.exists() and key.read_text() == built_for):
         return

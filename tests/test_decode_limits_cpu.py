@@ -91,3 +91,16 @@ def test_the_extension_is_built_anew_for_another_torch(pyext_builds, monkeypatch
     build._build_pyext()
     build._build_pyext()
     assert len(pyext_builds) == 2
+
+
+def test_the_library_is_built_without_torch(pyext_builds, monkeypatch, capsys):
+    """A C program's user needs the library alone."""
+    from aps2026_b200 import build
+
+    def version(name):
+        raise build.metadata.PackageNotFoundError(name)
+
+    monkeypatch.setattr(build.metadata, "version", version)
+    build._build_pyext()
+    assert pyext_builds == [] and not build.PYEXT_LIB.exists()
+    assert "torch" in capsys.readouterr().err
