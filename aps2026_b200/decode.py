@@ -127,7 +127,7 @@ def moe_decode_gpu(x, logits, w_gate_up, w_down, out, quantum: float = ROUTER_SC
     if code is None:
         raise InvalidArgument(f"moe_decode: gates must be one of {sorted(_GATES)}")
     if ws is None:
-        if x.dim() != 2 or w_down.dim() != 3:
+        if not all(isinstance(t, torch.Tensor) for t in (x, w_down)) or x.dim() != 2 or w_down.dim() != 3:
             raise InvalidArgument("moe_decode: expected x [T, H] and w_down [E, H, I]")
         ws = MoeWorkspace(x.shape[0], w_down.shape[2], x.device)
     rc = _decode_calls.moe_decode(x, logits, w_gate_up, w_down, out, quantum, tie_eps, code, ws.buf, ws.bytes)

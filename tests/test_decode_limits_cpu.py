@@ -104,3 +104,14 @@ def test_the_library_is_built_without_torch(pyext_builds, monkeypatch, capsys):
     build._build_pyext()
     assert pyext_builds == [] and not build.PYEXT_LIB.exists()
     assert "torch" in capsys.readouterr().err
+
+
+def test_experts_without_a_workspace_refuse_what_is_no_tensor():
+    import torch
+
+    x = torch.zeros(2, 8)
+    for bad in (None, "x", [1.0]):
+        with pytest.raises(ops.InvalidArgument):
+            decode.moe_decode_gpu(bad, x, x, x.view(2, 2, 4), x)
+        with pytest.raises(ops.InvalidArgument):
+            decode.moe_decode_gpu(x, x, x, bad, x)
