@@ -411,16 +411,16 @@ __device__ __forceinline__ void affine_operand(float q_sum, unsigned c, unsigned
     operand[1] = c < G ? p[2] : 0u;
 }
 
-// s < 2^(exponent - 126) for the largest s; the reference that puts p s of
-// score `top` (scaled) into [2^10, 2^11).
-__device__ __forceinline__ float reference_for(float top, float q_scale, unsigned exponent) {
-    return fmaf(top, q_scale, static_cast<float>(max(static_cast<int>(exponent) - 137, -71)));
+// What a step s < 2^(exponent - 126) asks of the reference above the score (in
+// base 2): p s in [2^10, 2^11) there.
+__device__ __forceinline__ float above_score(unsigned exponent) {
+    return static_cast<float>(max(static_cast<int>(exponent) - 137, -71));
 }
-// The same for one key, by its own parameters. A minimum counts as a step 2^80
-// below it, which keeps sums of p m over 2^28 keys in fp32 where steps are tiny
-// or zero; what is not finite has no part in it.
+// What one key's parameters ask. A minimum counts as a step 2^80 below it, which
+// keeps sums of p m over 2^28 keys in fp32 where steps are tiny or zero; what is
+// not finite has no part in it.
 template <unsigned G>
-__device__ __forceinline__ float reference_for_key(float x, float q_scale, const unsigned* params) {
+__device__ __forceinline__ float above_score_of(const unsigned* params) {
     int exponent = 0;
 #pragma unroll
     for (unsigned g = 0; g < G; ++g) {
@@ -428,15 +428,16 @@ __device__ __forceinline__ float reference_for_key(float x, float q_scale, const
         if (s != 0xFF) exponent = max(exponent, s);
         if (m != 0xFF) exponent = max(exponent, m - 80);
     }
-    return reference_for(x, q_scale, static_cast<unsigned>(exponent));
+    return above_score(static_cast<unsigned>(exponent));
 }
 // Minima from here on may need that; below it p m is in range whatever the
-// steps are (p < 2^75 at the least step reference_for counts).
+// steps are (p < 2^75 at the least step that above_score counts).
 constexpr float kLargeMinimum = 1048576.0f;
-// max(top, |m|) of a parameter word: m is the word's high half, so the word is
-// m but for its last bits.
-__device__ __forceinline__ float max_minimum(float top, unsigned params) {
-    return fmaxf(top, fabsf(__uint_as_float(params)));
+constexpr unsigned kLargeFlag = 0x8000u;  // beside a step's exponent
+// The larger |m| of two parameter words: m is the word's high half, so the word
+// is m but for its last bits.
+__device__ __forceinline__ float larger_minimum(unsigned params0, unsigned params1) {
+    return fmaxf(fabsf(__uint_as_float(params0)), fabsf(__uint_as_float(params1)));
 }
 
 __device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, unsigned tok, int j, int pos) {
@@ -486,6 +487,12 @@ struct Wide {
     // clear: every row sees all of the keys.
     __device__ __forceinline__ void step(const AttnKv4Args& a, const Tile& t, const Smem<D>& sm, unsigned stage,
                                          unsigned u0, unsigned valid, bool clear) {
+        // the step's largest s, and whether a minimum is large: a key per lane
+        unsigned own[G];
+        lds_n<G>(stage + 2 * S::codes + S::params + lane * 4 * G, own);
+        const unsigned steps_top = __reduce_max_sync(
+            0xffffffffu, ((G == 2 ? __vmaxu2(own[0], own[G - 1]) : own[0]) & 0x7F80u) |
+                             (larger_minimum(own[0], own[G - 1]) >= kLargeMinimum ? kLargeFlag : 0u));
         // ---- scores: x[b] holds keys 8b + 2c and 8b + 2c + 1 of row r ----
         f32x2 x[4];
         {
@@ -552,30 +559,28 @@ struct Wide {
         }
 
         // ---- the reference: p s is to stay below 2^15 ----
-        // A thread packs p s of its own keys only, so each tests its own, the top
-        // score against the largest step first. Only where that may be too much
-        // are keys taken one by one, each score with its own steps -- a large step
+        // A thread packs p s of its own keys only, so each tests its own, its top
+        // score against the step's largest s first. Only where that may be too
+        // much are keys taken one by one, each score with its own s -- a large s
         // of a key that the row does not see, or gives no weight, must not raise
         // the reference: the others' p s would sink below fp16 -- and exchanged.
-        float top = kNegInf, top_m = 0.0f;
-        unsigned top_w = vp[0][0];  // maxima of both halves of the words: s is the lower
+        // (A key's parameters are taken apart by one lane and passed on: 12
+        // sequences x 5 tokens 27.1 us; each thread with its own eight, 28.2.)
+        float top = kNegInf;
 #pragma unroll
         for (unsigned b = 0; b < 4; ++b) {
             const float2 y = f2_unpack(x[b]);
             top = fmaxf(top, fmaxf(y.x, y.y));
-#pragma unroll
-            for (unsigned i = 0; i < 2 * G; ++i) {
-                top_w = __vmaxu2(top_w, vp[b][i]);
-                top_m = max_minimum(top_m, vp[b][i]);
-            }
         }
-        float need = reference_for(top, q_scale, top_w >> 7 & 0xFFu);
-        if (__any_sync(0xffffffffu, need > ref + 4.0f || top_m >= kLargeMinimum)) {
+        float need = fmaf(top, q_scale, above_score(steps_top >> 7 & 0xFFu));
+        if (__any_sync(0xffffffffu, need > ref + 4.0f) || steps_top & kLargeFlag) {
             need = kNegInf;
+            const float above = above_score_of<G>(own);
 #pragma unroll
             for (unsigned b = 0; b < 4; ++b) {
                 const float2 y = f2_unpack(x[b]);
-                need = fmaxf(need, fmaxf(reference_for_key<G>(y.x, q_scale, vp[b]), reference_for_key<G>(y.y, q_scale, vp[b] + G)));
+                need = fmaxf(need, fmaf(y.x, q_scale, __shfl_sync(0xffffffffu, above, 8 * b + 2 * c)));
+                need = fmaxf(need, fmaf(y.y, q_scale, __shfl_sync(0xffffffffu, above, 8 * b + 2 * c + 1)));
             }
             need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 1));
             need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, 2));
@@ -800,13 +805,13 @@ struct Narrow {
             const float top0 = fmaxf(x0.x, x1.x), top1 = fmaxf(x0.y, x1.y);
             unsigned top_w = __vmaxu2(vp[0][0], vp[1][0]);  // maxima of both halves: s is the lower
             if (G == 2) top_w = __vmaxu2(top_w, __vmaxu2(vp[0][G - 1], vp[1][G - 1]));
-            const unsigned exponent = top_w >> 7 & 0xFFu;
-            float top_m = max_minimum(max_minimum(0.0f, vp[0][0]), vp[1][0]);
-            if (G == 2) top_m = max_minimum(max_minimum(top_m, vp[0][G - 1]), vp[1][G - 1]);
-            float need0 = reference_for(top0, scale.x, exponent), need1 = reference_for(top1, scale.y, exponent);
+            const float above = above_score(top_w >> 7 & 0xFFu);
+            const float top_m = fmaxf(larger_minimum(vp[0][0], vp[1][0]), larger_minimum(vp[0][G - 1], vp[1][G - 1]));
+            float need0 = fmaf(top0, scale.x, above), need1 = fmaf(top1, scale.y, above);
             if (__any_sync(0xffffffffu, need0 > old.x + 4.0f || need1 > old.y + 4.0f || top_m >= kLargeMinimum)) {
-                need0 = fmaxf(reference_for_key<G>(x0.x, scale.x, vp[0]), reference_for_key<G>(x1.x, scale.x, vp[1]));
-                need1 = fmaxf(reference_for_key<G>(x0.y, scale.y, vp[0]), reference_for_key<G>(x1.y, scale.y, vp[1]));
+                const float above0 = above_score_of<G>(vp[0]), above1 = above_score_of<G>(vp[1]);
+                need0 = fmaxf(fmaf(x0.x, scale.x, above0), fmaf(x1.x, scale.x, above1));
+                need1 = fmaxf(fmaf(x0.y, scale.y, above0), fmaf(x1.y, scale.y, above1));
 #pragma unroll
                 for (unsigned i = 2; i < 32; i *= 2) {
                     need0 = fmaxf(need0, __shfl_xor_sync(0xffffffffu, need0, i));
