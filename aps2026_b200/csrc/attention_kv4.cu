@@ -21,26 +21,32 @@
 // O^T += V^T P^T. Two forms of a tile of rows (heads x new tokens of one KV
 // head): Wide, 8 rows, and Narrow, 4 rows, which a single token of a group of
 // up to 4 heads takes, and where hi and lo parts share an instruction's
-// columns (64 sequences of 4095 .. 32768 positions, 4 KV heads of 4 heads
-// each: 167 us, Wide with half of its rows empty 214).
+// columns (64 sequences of 4095 .. 32768 positions, 4 KV heads of 4 heads each:
+// 178 us; with the same inputs in a row, partly from L2, 166, and 219 in Wide,
+// half of its rows empty).
 //
 // The steps of all (row tile, KV head) pairs are cut into equal shares, one
 // per CTA, two CTAs per SM, so that ragged lengths and one long sequence load
 // every SM alike. When there are no more pairs than CTAs, each pair gets CTAs
 // of its own, unless that leaves some CTA with 28 steps more than its share:
 // a CTA with parts of two pairs pays a part's latencies twice (32 sequences of
-// 129 .. 4096 positions, window 2047: 18.6 us, as one list 27.2; 16 of 4095 ..
-// 32768 with 8 KV heads 117 and 113). A pair's parts
+// 129 .. 4096 positions, window 2047: 18.5 us, as one list 27.4; 16 of 4095 ..
+// 32768, two tokens on 8 KV heads of 4 heads: 3 us more than as one list, of
+// 115). A pair's parts
 // meet in the workspace, where the last CTA to arrive adds them in the
 // order of their keys, so results repeat bit for bit.
 //
-// What bounds it: with long contexts, instruction issue. 144 bytes per
-// position and KV head (head_dim 128) would be 105 us of HBM time for the 679
-// MB of 64 sequences; the step's some 700 instructions (half of them turn
-// nibbles into fp16) take 167 to 178 (issue 63% active, ALU 56%, matrix unit 24%,
-// DRAM 3.9 TB/s). With little work per CTA, the chain of latencies: lengths,
-// page numbers, keys, the warps' meeting, the parts' meeting (31 us for one
-// sequence of 131,069, 11.7 us of HBM time; 7 us for one of 37).
+// What bounds it: with long contexts, the step's some 700 instructions (half
+// of them turn nibbles into fp16) in 16 warps per SM at 128 registers, each of
+// which runs QK, softmax and PV one after the other. 144 bytes per position and
+// KV head (head_dim 128) would be 105 us of HBM time for the 679 MB of 64
+// sequences; it takes 178, with issue 64% active, ALU 56%, matrix unit 24%, DRAM 3.8
+// TB/s: no unit is at its limit, there is too little independent work. With
+// little work per CTA, the chain of latencies: lengths, page numbers, keys, the
+// warps' meeting, the parts' meeting (33 us for one sequence of 131,069, 11.7 us
+// of HBM time; 7 us for one of 37). With the rows of a whole prompt, many short
+// parts: shares count steps, so the CTA with a prompt's first rows gets some 200
+// parts of 1 to 4 steps (2048 rows over 2048 positions 1038 us, over 8192 1287).
 #include <algorithm>
 #include <cmath>
 
@@ -330,7 +336,9 @@ __device__ __forceinline__ unsigned mask_or(unsigned w, unsigned mask, unsigned 
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(bits));
     return d;
 }
-// c - 8 of the low (SHIFTED: second) nibbles of both halves of w, in fp16.
+// c - 8 of the low (SHIFTED: second) nibbles of both halves of w, in fp16: the
+// conversion by fp16's exponent that Kim et al. published ("Who Says Elephants
+// Can't Run", 2022), whose constants follow from the format.
 template <bool SHIFTED>
 __device__ __forceinline__ unsigned codes_f16(unsigned w) {
     unsigned d;
@@ -446,7 +454,7 @@ __device__ __forceinline__ bool visible(const AttnKv4Args& a, unsigned valid, un
 }
 
 // Eight rows (5 new tokens of 4 heads on each of 4 KV heads, 12 sequences of
-// 500 .. 4000: 27.5 us). Queries are the M = 16 operand of QK (hi parts in rows 0..7, lo
+// 500 .. 4000: 27.1 us). Queries are the M = 16 operand of QK (hi parts in rows 0..7, lo
 // in 8..15), so thread (r, c) gets the scores of row r and keys 8b + 2c, + 1,
 // which is where the second product wants P^T (k = keys, n = rows).
 template <unsigned D>

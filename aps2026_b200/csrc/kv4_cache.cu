@@ -13,10 +13,12 @@
 // exchange, and the groups' minima and maxima are shuffles inside the
 // subgroup. One launch covers the row's q, k and v heads, in a grid-stride
 // loop of all the CTAs that the SMs hold: 13,547 rows of 16 q and 2 x 4 kv
-// heads of a fused projection appended and read back in 66.8 us, 356 MB at 82%
-// of the measured copy rate; what is left is the wait for each loop's loads
-// (long_scoreboard: 12 of 19 cycles between two instructions of a warp). For a
-// decode step's few rows the two calls cost their launches, 6 us.
+// heads of a fused projection appended and read back in 67 us, 356 MB at 82%
+// of the measured copy rate. The append takes 46 us of it, 98%; the read 17, 57%:
+// each 8 values wait for row, page and code word in turn, and a row's K and V
+// look their page up separately (long_scoreboard: 23 cycles between two
+// instructions of a warp). In bf16 47 us, 62% (33 and 12). For a decode step's few
+// rows the two calls cost their launches: 5 to 8 us, by the host.
 #include "kv4.cuh"
 
 namespace b2 {

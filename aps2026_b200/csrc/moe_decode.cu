@@ -17,8 +17,8 @@
 // bf16 weights meet fp32 activations as three bf16 parts (24 bits), fp32
 // weights as TF32 hi and lo (hi hi + hi lo + lo hi). Its accumulator
 // truncates, a bias that grows with the chain, so a chain is one block long
-// and blocks are added in registers (61 tokens in fp32: error 6.5e-7 of the
-// output and 84 us; two blocks per chain 9.6e-7 and 88).
+// and blocks are added in registers (61 tokens in fp32: error 6.6e-7 of the
+// output; two blocks per chain 9.6e-7, and 4 us more).
 //
 // Launch 1, moe_gate_up: an item is (expert with up to 8 NT of its tokens,
 // 8 MT rows of gate and the same of up); a CTA takes equally many items, one
@@ -32,12 +32,13 @@
 // routed and requested its first weights before it waits.
 //
 // What bounds it: one token, the two launches' latencies (routing, first
-// weights, the meeting, the hand-over: 12.4 us at 4096 x 448 x 16 in bf16,
-// 3.4 us of HBM time). 9 tokens, HBM with those latencies (27 us, 19 of HBM
-// time). 61 tokens in fp32, instruction issue: splitting weights into TF32
-// parts and three products each (launch 1: 64 us, issue 55% active, matrix
-// unit 31%, no stall on memory; both 87, HBM time 55). 128 tokens, splitting
-// the activations anew for every 16 rows (41 us at 1001 x 333 x 7).
+// weights, the meeting, the hand-over: 12.7 us at 4096 x 448 x 16 in bf16,
+// 3.4 us of HBM time). 9 tokens, HBM with those latencies (27 to 31 us, 19 of
+// HBM time). 61 tokens in fp32, fixed latencies: weights split into TF32 parts
+// and chains of three products each, in 16 warps per SM (launch 1: 60 us, issue
+// 54% active, matrix unit 35%; both 88, HBM time 55). 128 tokens, splitting
+// the activations anew for every 16 rows (41 us at 1001 x 333 x 7; at 4096 x 448
+// x 16 85, HBM time 28, and 67 with bf16 activations, which are not split).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -998,7 +999,7 @@ cudaError_t launch_moe(const MoeDecodeArgs& a, cudaStream_t s) {
     const bool vec_down = a.I % kPer<W> == 0 && aligned16(a.w_down);
     // 16 tokens per group, and 16 rows of gate and up per item, where the
     // experts have more than 4 tokens on average: fewer experts are read twice,
-    // fewer activations split twice (128 tokens of 4096 x 448 x 16: 87 us, with
+    // fewer activations split twice (128 tokens of 4096 x 448 x 16: 85 us, with
     // 8 rows 107); else 8 of each, whose smaller stages leave more weights in flight
     const bool wide = 2 * a.T > 4 * a.E;
     cudaError_t e = vec_up ? wide ? launch_up<X, W, 2, 2, true>(a, s) : launch_up<X, W, 1, 1, true>(a, s)

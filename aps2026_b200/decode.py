@@ -54,7 +54,8 @@ def kv4_append_gpu(k, v, row_seq, row_pos, cache: KVCache4, page_table, q=None, 
     """Appends rows to the cache (b2_kv4_append): keys rotated at row_pos and
     rounded to 4 bits, values rounded, stored at (row_seq, row_pos); with q,
     q_out = the rotated queries. k, v: [rows, kv_heads, head_dim], q and q_out
-    [rows, q_heads, head_dim], fp32 or bf16; cos, sin: the fp32 tables
+    [rows, q_heads, head_dim], fp32 or bf16, q_out contiguous and 16-byte
+    aligned; cos, sin: the fp32 tables
     [positions, head_dim / 2] of rope_table_host on the device, or None for no
     rotation. row_seq = PADDING marks a row that is not there."""
     rc = _decode_calls.kv4_append(k, v, row_seq, row_pos, cache.data, cache.pages, cache.page_size, cache.kv_heads,
@@ -64,9 +65,9 @@ def kv4_append_gpu(k, v, row_seq, row_pos, cache: KVCache4, page_table, q=None, 
 
 
 def kv4_read_gpu(cache: KVCache4, page_table, row_seq, row_pos, k_out, v_out) -> None:
-    """k_out, v_out [rows, kv_heads, head_dim] = the values the cache holds at
-    (row_seq, row_pos) (b2_kv4_read), e.g. the K and V of a cached prefix for
-    attention_tree_gpu."""
+    """k_out, v_out [rows, kv_heads, head_dim], contiguous and 16-byte aligned,
+    = the values the cache holds at (row_seq, row_pos) (b2_kv4_read), e.g. the K
+    and V of a cached prefix for attention_tree_gpu."""
     rc = _decode_calls.kv4_read(cache.data, cache.pages, cache.page_size, cache.kv_heads, cache.head_dim, page_table,
                                 row_seq, row_pos, k_out, v_out)
     if rc:
@@ -89,8 +90,8 @@ def attention_kv4_gpu(q, cache: KVCache4, page_table, lens, out, q_offsets=None,
                       ws: AttentionWorkspace | None = None) -> None:
     """out = attention of each sequence's newest query rows over its cached
     keys and values (b2_attention_kv4). q, out: [rows, q_heads, head_dim],
-    fp32 or bf16; lens [seqs] counts the cached positions, the query rows'
-    own among them; q_offsets [seqs + 1] splits the rows between the sequences
+    fp32 or bf16, out contiguous and 16-byte aligned; lens [seqs] counts the
+    cached positions, the query rows' own among them; q_offsets [seqs + 1] splits the rows between the sequences
     (None: one row each). Key j is visible at position p when j <= p and
     (p - j < window or j < sinks); window 0: no window. max_queries and
     max_len (default: the page table's reach) bound a sequence's query rows

@@ -404,7 +404,8 @@ int b2_kv4_page_bytes(size_t page_size, size_t kv_heads, size_t head_dim, size_t
  * q, k, v: `dtype`, [rows, heads, head_dim] with strides in elements between
  * rows and between heads (the dimensions of a head adjacent), so slices of a
  * fused projection need no copy; q_out: `dtype`, [rows, q_heads, head_dim]
- * contiguous, may be q when q is contiguous. Rows must not share a position.
+ * contiguous and 16-byte aligned, may be q when q is so. Rows must not share a
+ * position.
  * Reported through b2_device_status and skipped (q_out zero where the
  * rotation could not be had): a position past table_rows (B2_CHECK_ROPE); a
  * sequence, position or page outside the cache (B2_CHECK_KV4). q_out of
@@ -421,9 +422,10 @@ int b2_kv4_append(const void* q, size_t q_row_stride, size_t q_head_stride,
 
 /*
  * Reads rows back as the values the cache holds: k_out, v_out ([rows,
- * kv_heads, head_dim] contiguous, `dtype`) = the keys and values at
- * (row_seq[r], row_pos[r]); what the tree attention of a prompt that
- * continues a cached prefix takes as K and V. Rows outside the cache are
+ * kv_heads, head_dim] contiguous and 16-byte aligned, `dtype`) = the keys and
+ * values at (row_seq[r], row_pos[r]); what the tree attention of a prompt that
+ * continues a cached prefix takes as K and V (the prefix's rows and the
+ * prompt's own, with any queries on the prefix's). Rows outside the cache are
  * reported (B2_CHECK_KV4) and zero; padding rows (0xFFFFFFFF) are zero.
  */
 int b2_kv4_read(const b2_kv4_cache* cache, const uint32_t* row_seq,
@@ -442,14 +444,19 @@ int b2_kv4_read(const b2_kv4_cache* cache, const uint32_t* row_seq,
  * window == 0: every j <= p. A row that sees no key is zero. Pages of keys
  * that no row sees are not touched.
  * q: `dtype` with strides as in b2_kv4_append; out: `dtype`, [rows, q_heads,
- * head_dim] contiguous. max_queries and max_len bound the query rows and the
- * length of a sequence (they size the launch).
+ * head_dim] contiguous and 16-byte aligned. max_queries and max_len bound the
+ * query rows and the length of a sequence (they size the launch).
+ * Accuracy: as of fp32 sums for keys and values of 2^-70 to 2^100 in size, if
+ * the steps of a value's two halves (head_dim 128) are within 2^12 of each
+ * other; what a row does not see, or gives no weight, does not matter. Past
+ * these bounds bits are lost, the smaller half's first.
  * workspace: b2_attention_kv4_workspace_size bytes, 16-byte aligned, all zero
  * before its first use; every call leaves it ready for the next. Calls that
  * overlap on the GPU must not share it.
  * Limits: max_len <= 2^28; max_queries * q_heads < 2^31; with up to 8 query
  * rows of a KV head per row tile, seqs * tiles * kv_heads * max_len < 2^35.
- * scale must be finite; 0 and below are allowed.
+ * scale must be finite; 0 and below are allowed. A window of max_len or more
+ * is none.
  * Reported through b2_device_status (B2_CHECK_KV4): a sequence with more
  * than max_queries query rows or offsets outside [0, rows] (its rows are not
  * written); a length above max_len or the table's reach (its rows are zero);
@@ -478,7 +485,10 @@ int b2_attention_kv4(const void* q, size_t q_row_stride, size_t q_head_stride,
  * x [T, ld_x >= H] and out [T, ld_out >= H]: x_dtype; logits [T, E] fp32,
  * 2 <= E <= 32; w_gate_up [E, 2I, H] and w_down [E, H, I] contiguous:
  * w_dtype, aligned to their element at least (rows and tensors aligned to 16
- * bytes are faster). Sums in fp32; fp32 operands keep 22 bits or more.
+ * bytes are faster). Sums in fp32; fp32 operands keep 22 bits or more (weights
+ * of less than 2^-100 fewer). An infinite operand, or one at the end of its
+ * type, gives what a plain fp32 sum gives; sums that it makes NaN are taken
+ * again one by one, which costs time.
  * out may not overlap x. T > 128: B2_ERR_UNSUPPORTED (route with
  * b2_moe_route and run the experts as grouped products).
  * workspace: b2_moe_decode_workspace_size bytes, 16-byte aligned; no

@@ -310,3 +310,48 @@ def test_experts_are_those_of_the_routing(cuda, E, spread):
         decode.moe_decode_gpu(x, logits, gate_up, down, out)
         want = torch.zeros(T, 32, device="cuda").scatter_(1, ops.moe_route_gpu(logits).routes.long(), 1.0)
         assert torch.equal((out != 0).float(), want)
+
+
+@pytest.mark.parametrize("q_heads", [4, 16])
+@pytest.mark.parametrize("dim,key,first,second", [(64, 0, -70, 0), (64, 0, 100, 0), (64, 100, 0, 0), (64, -70, 0, 0), (128, 0, 0, 12),
+                                                  (128, 0, 12, 0), (128, 0, -70, -58), (128, 0, 100, 88), (128, 100, 100, 100)])
+def test_attention_in_the_stated_range(cuda, q_heads, dim, key, first, second):
+    """Keys 2^key, values' halves 2^first and 2^second times the usual size:
+    each half as close as at the usual size."""
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g, n, kv_heads = _gen(dim), 1500, 2
+    cache, table, k, v = _filled(g, [n], 16, kv_heads, dim)
+    k *= 2.0 ** key
+    v[..., :64] *= 2.0 ** first
+    v[..., 64:] *= 2.0 ** second
+    seq, pos = _i32([0] * n), torch.arange(n, device="cuda", dtype=torch.int32)
+    decode.kv4_append_gpu(k, v, seq, pos, cache, table)
+    decode.kv4_read_gpu(cache, table, seq, pos, k, v)
+    q, out = _randn(g, 1, q_heads, dim) * 2.0 ** -key, torch.empty(1, q_heads, dim, device="cuda")
+    decode.attention_kv4_gpu(q, cache, table, _i32([n]), out)
+    want = _one_row64(q, k, v, dim ** -0.5)
+    for part in range(0, dim, 64):
+        a, b = out[..., part:part + 64].double(), want[..., part:part + 64]
+        assert float((a - b).norm() / b.norm()) < ROW
+    assert ops.device_status() == 0
+
+
+def test_outputs_off_a_16_byte_boundary_are_refused(cuda):
+    import torch
+
+    from aps2026_b200 import decode, ops
+
+    g = _gen(4)
+    cache, table, k, v = _filled(g, [3], 8, 1, 64)
+    off = torch.empty(1 + 3 * 64, device="cuda")[1:].view(3, 1, 64)
+    seq, pos, q = _i32([0] * 3), _i32([0, 1, 2]), _randn(g, 3, 1, 64)
+    for call in (lambda: decode.kv4_append_gpu(k, v, seq, pos, cache, table, q=q, q_out=off),
+                 lambda: decode.kv4_read_gpu(cache, table, seq, pos, off, v),
+                 lambda: decode.kv4_read_gpu(cache, table, seq, pos, k, off),
+                 lambda: decode.attention_kv4_gpu(q, cache, table, _i32([3]), off, q_offsets=_i32([0, 3]), max_queries=3)):
+        with pytest.raises(ops.InvalidArgument, match="16-byte"):
+            call()
+    assert ops.device_status() == 0
